@@ -165,6 +165,96 @@ uint64_t syn_hip_attend_batch_scratch_bytes(const syn_seq_desc* seqs, uint32_t n
 int syn_hip_attend_batch(syn_arena* arena, const syn_seq_desc* seqs, uint32_t n_seqs, uint32_t n_heads,
                          float scale, uint32_t q_dtype, uint64_t scratch_offset, uint64_t scratch_bytes);
 
+/* ---- 8-bit KV states --------------------------------------------------------
+ * No reference counterpart: the reference's cache is binary16. A state at
+ * half the size: each row (position, KV head) of K and of V is head_dim
+ * whole numbers q in -127..127 and one f32 step d,
+ *   d = max|x| / 127 (rounded to f32),  q = x / d to the nearest whole
+ * number, ties to even, and stands for the values q * d. A row of zeros has
+ * step 0; a row with an infinity or NaN stands for NaN throughout, and makes
+ * NaN of the outputs that attend it and of no others. The bytes' order in
+ * the arena is the library's own; nothing in a state needs to start at
+ * zero. Positions, heads and limits as for syn_kv_desc, with max_ctx at most
+ * 2^31 - 64. */
+typedef struct syn_kv8_desc {
+    uint64_t offset;     /* syn_hip_kv8_state_bytes() bytes, 256-byte aligned */
+    uint32_t max_ctx;
+    uint32_t n_kv_heads;
+    uint32_t head_dim;   /* even, <= 256 */
+    uint32_t reserved;
+} syn_kv8_desc;
+
+/* Bytes of one state (0 for a shape that no state can have). */
+uint64_t syn_hip_kv8_state_bytes(uint32_t max_ctx, uint32_t n_kv_heads, uint32_t head_dim);
+
+/* Positions pos0..pos0+n-1 <- the n rows of n_kv_heads*head_dim at k_rows and
+ * v_rows (type kv_dtype), quantized. Other positions stay as they are. The
+ * rows may not overlap the state. */
+int syn_hip_kv8_append(syn_arena* arena, const syn_kv8_desc* cache, uint64_t k_rows, uint64_t v_rows, uint32_t n,
+                       uint32_t pos0, uint32_t kv_dtype);
+
+/* The values of positions pos0..pos0+n-1 as n rows of n_kv_heads*head_dim at
+ * k_out and v_out (type out_dtype): q * d rounded to f32, and that to
+ * binary16 for SYN_F16. The rows may overlap neither the state nor each
+ * other. */
+int syn_hip_kv8_read(syn_arena* arena, const syn_kv8_desc* cache, uint64_t k_out, uint64_t v_out, uint32_t n,
+                     uint32_t pos0, uint32_t out_dtype);
+
+/* Attention over an 8-bit state: syn_hip_attention's formula with the state's
+ * values for K and V. q is rounded to binary16 first, as there; everything
+ * after that keeps f32's range and at least 20 bits. With a mask, the run's
+ * n rows are a drafted tree instead of a sequence: see syn_hip_attend_tree. */
+typedef struct syn_kv8_attn_desc {
+    syn_kv8_desc cache;
+    uint64_t q_offset;       /* n rows of n_heads*head_dim, type q_dtype */
+    uint64_t k_offset;       /* n rows of n_kv_heads*head_dim, type kv_dtype (syn_hip_kv8_attention) */
+    uint64_t v_offset;
+    uint64_t out_offset;     /* n rows of n_heads*head_dim f32 */
+    uint64_t scratch_offset; /* see syn_hip_kv8_attention_scratch_bytes; 16-byte aligned */
+    uint64_t scratch_bytes;
+    uint64_t mask_offset;    /* a tree's mask, or UINT64_MAX: a causal run */
+    uint32_t n_heads;        /* a multiple of cache.n_kv_heads */
+    uint32_t pos;            /* position of the run's first token */
+    uint32_t n;              /* tokens, >= 1; pos + n <= cache.max_ctx */
+    float scale;             /* finite, > 0 */
+    uint32_t q_dtype;
+    uint32_t kv_dtype;
+} syn_kv8_attn_desc;
+
+/* Scratch for calls of up to max_batch tokens on a state of max_ctx. */
+uint64_t syn_hip_kv8_attention_scratch_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                             uint32_t max_ctx, uint32_t max_batch);
+/* Appends the run's n rows, then attends (syn_hip_attention's two halves), */
+int syn_hip_kv8_attention(syn_arena* arena, const syn_kv8_attn_desc* desc);
+/* or attends only: positions 0..pos+n-1 are in the state (k_offset and
+ * v_offset are ignored). */
+int syn_hip_kv8_attend(syn_arena* arena, const syn_kv8_attn_desc* desc);
+
+/* ---- drafted trees ------------------------------------------------------------
+ * No reference counterpart. A step that verifies n drafted tokens at once:
+ * their K, V rows are appended at positions pos..pos+n-1, in any order (rows
+ * of one depth next to each other take one syn_hip_rope call with period 1),
+ * then token i attends positions 0..pos-1 and those drafted tokens j whose
+ * bit is set in row i of the mask -- its ancestors and itself. The mask is n
+ * rows of (n + 31) / 32 32-bit words in the arena, bit j % 32 of word j / 32
+ * (bits from n on are ignored), 4-byte aligned; any pattern is allowed. What
+ * a token does not attend has no part in its output, infinities and NaN
+ * included; a token that attends nothing (pos 0, no bit) gets zeros. K, V and
+ * the formula as in syn_hip_attend, with the probabilities kept to 22 bits;
+ * desc's k_offset and v_offset are ignored. */
+uint64_t syn_hip_attend_tree_scratch_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                           uint32_t max_ctx, uint32_t max_batch);
+int syn_hip_attend_tree(syn_arena* arena, const syn_attn_desc* desc, uint64_t mask_offset);
+
+/* After it, the accepted tokens' rows moved to the front of the drafted ones:
+ * position pos + i <- position pos + rows[i] for i < count, rows (host
+ * memory) rising and below n, n at most 65536. Other positions stay as they
+ * are. */
+int syn_hip_kv_keep(syn_arena* arena, const syn_kv_desc* cache, uint32_t pos, uint32_t n, const uint32_t* rows,
+                    uint32_t count);
+int syn_hip_kv8_keep(syn_arena* arena, const syn_kv8_desc* cache, uint32_t pos, uint32_t n, const uint32_t* rows,
+                     uint32_t count);
+
 /* ---- bidirectional self-attention (image encoders) ----------------------
  * session::execute(op_self_attention) (S/graph/session.hpp:409-449) with
  * self_attend_head's math (S/kernels/attention.hpp:460-486): for every row i

@@ -48,7 +48,7 @@ HIP_FLAGS = [
 # same for the decode kernel measured no change.
 SOURCE_FLAGS = {"quant_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                 "matmul_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
-HIP_SOURCES = ["kv_append.hip", "decode.hip", "prefill.hip", "flash.hip", "flash_f32.hip", "generic.hip", "rope.hip", "ops.hip",
+HIP_SOURCES = ["attend_kv8.hip", "attend_tree.hip", "attend_merge.hip", "kv8.hip", "kv_append.hip", "decode.hip", "prefill.hip", "flash.hip", "flash_f32.hip", "generic.hip", "rope.hip", "ops.hip",
                "matmul_f32.hip",
                "quant.hip", "quant_gemm.hip", "capi.hip"]
 
@@ -97,7 +97,8 @@ CPP_TESTS = {
 }
 # Host builds of device-side math, layouts and launch rules (no library, no HIP).
 CPP_MATH_TESTS = {name: f"tests/cpp/{name}.cpp"
-                  for name in ("test_rope_math", "test_decode_lds", "test_matmul_f32_plan", "test_quant_plan")}
+                  for name in ("test_rope_math", "test_decode_lds", "test_matmul_f32_plan", "test_quant_plan",
+                               "test_attend_rows_plan")}
 # Host tests linked against tests/cpp/stub_abi.cpp (a C ABI that launches
 # nothing) instead of the library: they run on the CPU.
 CPP_STUB_TESTS = {"test_no_alloc": "tests/cpp/test_no_alloc.cpp"}

@@ -97,6 +97,16 @@ class SoftmaxDesc(ctypes.Structure):
     _fields_ = [("in_offset", u64), ("out_offset", u64), ("n", u32), ("size", u32)]
 
 
+class Kv8Desc(ctypes.Structure):
+    _fields_ = [("offset", u64), ("max_ctx", u32), ("n_kv_heads", u32), ("head_dim", u32), ("reserved", u32)]
+
+
+class Kv8AttnDesc(ctypes.Structure):
+    _fields_ = [("cache", Kv8Desc), ("q_offset", u64), ("k_offset", u64), ("v_offset", u64), ("out_offset", u64),
+                ("scratch_offset", u64), ("scratch_bytes", u64), ("mask_offset", u64), ("n_heads", u32),
+                ("pos", u32), ("n", u32), ("scale", f32), ("q_dtype", u32), ("kv_dtype", u32)]
+
+
 SYN_ADD, SYN_MUL, SYN_SILU_MUL, SYN_SCALE, SYN_GELU, SYN_SILU, SYN_ADD_BIAS = 0, 1, 2, 3, 4, 5, 6
 
 
@@ -123,6 +133,16 @@ SIGNATURES = {
     "syn_hip_kv_append": (i32, [ctypes.c_void_p, ctypes.POINTER(KvDesc), u64, u64, u32, u32, u32]),
     "syn_hip_attend_batch_scratch_bytes": (u64, [ctypes.POINTER(SeqDesc), u32, u32]),
     "syn_hip_attend_batch": (i32, [ctypes.c_void_p, ctypes.POINTER(SeqDesc), u32, u32, f32, u32, u64, u64]),
+    "syn_hip_kv8_state_bytes": (u64, [u32, u32, u32]),
+    "syn_hip_kv8_append": (i32, [ctypes.c_void_p, ctypes.POINTER(Kv8Desc), u64, u64, u32, u32, u32]),
+    "syn_hip_kv8_read": (i32, [ctypes.c_void_p, ctypes.POINTER(Kv8Desc), u64, u64, u32, u32, u32]),
+    "syn_hip_kv8_attention_scratch_bytes": (u64, [u32, u32, u32, u32, u32]),
+    "syn_hip_kv8_attention": (i32, [ctypes.c_void_p, ctypes.POINTER(Kv8AttnDesc)]),
+    "syn_hip_kv8_attend": (i32, [ctypes.c_void_p, ctypes.POINTER(Kv8AttnDesc)]),
+    "syn_hip_attend_tree_scratch_bytes": (u64, [u32, u32, u32, u32, u32]),
+    "syn_hip_attend_tree": (i32, [ctypes.c_void_p, ctypes.POINTER(AttnDesc), u64]),
+    "syn_hip_kv_keep": (i32, [ctypes.c_void_p, ctypes.POINTER(KvDesc), u32, u32, ctypes.POINTER(u32), u32]),
+    "syn_hip_kv8_keep": (i32, [ctypes.c_void_p, ctypes.POINTER(Kv8Desc), u32, u32, ctypes.POINTER(u32), u32]),
     "syn_hip_self_attention": (i32, [ctypes.c_void_p, ctypes.POINTER(SelfDesc)]),
     "syn_hip_rope": (i32, [ctypes.c_void_p, ctypes.POINTER(RopeDesc)]),
     "syn_hip_attn_temperature": (i32, [ctypes.c_void_p, ctypes.POINTER(TemperatureDesc)]),
@@ -317,6 +337,31 @@ def kv_state(arena: Arena, max_ctx: int, n_kv: int, hd: int) -> KvDesc:
 
 def kv_state_bytes(max_ctx: int, n_kv: int, hd: int) -> int:
     return int(lib().syn_hip_kv_state_bytes(max_ctx, n_kv, hd))
+
+
+def kv8_state(arena: Arena, max_ctx: int, n_kv: int, hd: int) -> Kv8Desc:
+    """Places one 8-bit KV state in the arena."""
+    return Kv8Desc(offset=arena.alloc(kv8_state_bytes(max_ctx, n_kv, hd)), max_ctx=max_ctx, n_kv_heads=n_kv,
+                   head_dim=hd)
+
+
+def kv8_state_bytes(max_ctx: int, n_kv: int, hd: int) -> int:
+    return int(lib().syn_hip_kv8_state_bytes(max_ctx, n_kv, hd))
+
+
+def tree_mask(parents) -> np.ndarray:
+    """The mask of a drafted tree, as syn_hip_attend_tree takes it, from each
+    token's parent (an earlier token, or -1 for one right behind the cache):
+    bit j of row i is set where j is i or one of its ancestors."""
+    n = len(parents)
+    bits = np.zeros((n, (n + 31) // 32 * 32), dtype=bool)
+    for i, parent in enumerate(parents):
+        if not -1 <= parent < i:
+            raise ValueError(f"token {i}: parent {parent}")
+        if parent >= 0:
+            bits[i] = bits[parent]
+        bits[i, i] = True
+    return np.packbits(bits, axis=1, bitorder="little").view(np.uint32)
 
 
 def upload_cache(arena: Arena, c: KvDesc, k_rows16: np.ndarray, v_rows16: np.ndarray) -> None:

@@ -1,0 +1,135 @@
+// attend_rows_plan.hpp — how attend_rows (attend_rows.hpp) cuts a call into
+// blocks, and the layout of an 8-bit KV state. Plain host arithmetic (tests
+// build it without HIP).
+#pragma once
+
+#include <algorithm>
+#include <cstdint>
+
+namespace syn {
+
+// ---- 8-bit KV states --------------------------------------------------------
+// A KV head's positions in tiles of 64; a tile's record holds its K bytes, V
+// bytes, K steps and V steps. Bytes are value + 128 (attend_rows.hpp turns
+// them into halves by placing them in a mantissa).
+constexpr uint32_t kv8_tile = 64;
+
+struct kv8_shape {
+    uint32_t n_kv, hd;
+    uint32_t hdp;         // hd rounded up to whole 32s, the matrix core's k
+    uint32_t tiles;       // tiles of one KV head
+    uint32_t v_at;        // V bytes in a record (K bytes are at 0)
+    uint32_t ks_at;       // K steps
+    uint32_t vs_at;       // V steps
+    uint32_t tile_bytes;  // a record
+};
+
+inline kv8_shape kv8_shape_of(uint32_t max_ctx, uint32_t n_kv, uint32_t hd) {
+    kv8_shape s{};
+    s.n_kv = n_kv;
+    s.hd = hd;
+    s.hdp = (hd + 31) / 32 * 32;
+    s.tiles = max_ctx / kv8_tile + (max_ctx % kv8_tile != 0);
+    s.v_at = kv8_tile * s.hdp;
+    s.ks_at = 2 * kv8_tile * s.hdp;
+    s.vs_at = s.ks_at + kv8_tile * 4;
+    s.tile_bytes = s.vs_at + kv8_tile * 4;
+    return s;
+}
+
+inline uint64_t kv8_bytes(const kv8_shape& s) {
+    return uint64_t{s.n_kv} * s.tiles * s.tile_bytes;
+}
+
+// Where position key (of its tile), dim d has its K byte. A wave's load of a
+// score operand (16 keys x 64 dims, lane 16 G + m: 16 dims of key row m) is
+// 1 KiB in lane order; an odd last 32 dims take 8 bytes a lane. Row m = 4 G'
+// + r of operand (c, a) is key 32 c + 8 G' + 4 a + r, so that a lane's eight
+// scores of operands (c, 0) and (c, 1) are eight neighbouring keys, which is
+// how the output product wants its probabilities.
+inline constexpr uint32_t kv8_k_at(uint32_t hdp, uint32_t key, uint32_t d) {
+    const uint32_t c = key / 32, g = key / 8 % 4, a = key / 4 % 2, r = key % 4;
+    const uint32_t m = 4 * g + r;
+    const uint32_t base = (2 * c + a) * 16 * hdp;
+    const uint32_t pairs = hdp / 64 * 64;  // dims in whole 64s
+    if (d < pairs) {
+        return base + d / 64 * 1024 + (d % 64 / 16 * 16 + m) * 16 + d % 16;
+    }
+    const uint32_t e = d - pairs;
+    return base + pairs * 16 + (e / 8 * 16 + m) * 8 + e % 8;
+}
+// Its V byte: 16 dims x 64 keys are 1 KiB in lane order, lane 16 G + d % 16
+// holding keys 8 G .. + 7 and 32 + 8 G .. + 7.
+inline constexpr uint32_t kv8_v_at(uint32_t key, uint32_t d) {
+    return d / 16 * 1024 + (key / 8 % 4 * 16 + d % 16) * 16 + key / 32 * 8 + key % 8;
+}
+
+// ---- blocks of attend_rows --------------------------------------------------
+constexpr uint32_t attend_tile = 64;        // keys of a wave's step
+constexpr uint32_t attend_waves = 4;        // waves of a block; they share out its keys
+constexpr uint32_t attend_max_splits = 256;
+// Splits are added up to this many blocks (256 CUs, two blocks each).
+constexpr uint32_t attend_split_blocks = 512;
+
+struct attend_plan {
+    uint32_t row_tiles;    // 16-row tiles of query rows per block
+    uint32_t row_blocks;   // blocks over the query rows of one KV head
+    uint32_t chunk;        // key tiles per split
+    uint32_t splits;
+};
+
+// The most splits a plan of these row blocks may have on up to len keys.
+inline uint32_t attend_max_splits_of(const attend_plan& p, uint32_t n_kv, uint32_t len) {
+    const uint64_t units = uint64_t{p.row_blocks} * n_kv;
+    const uint32_t tiles = len / attend_tile + (len % attend_tile != 0);
+    const uint64_t few = units < attend_split_blocks ? attend_split_blocks / units : 1;
+    return static_cast<uint32_t>(std::min<uint64_t>(
+        {few, std::max(1u, tiles / attend_waves + (tiles % attend_waves != 0)), attend_max_splits}));
+}
+
+// n tokens of `group` query heads per KV head attend up to len keys.
+inline attend_plan plan_attend_rows(uint32_t n, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t len,
+                                    bool eight) {
+    attend_plan p{};
+    const uint64_t rows = uint64_t{n} * group;
+    // Rows' operands and outputs are registers: 64 rows fill them at hd 128.
+    // Binary16 K rows off 16 bytes are read by pairs, in 16-row blocks only.
+    const uint32_t most = !eight && hd % 8 != 0 ? 1 : hd > 128 ? 2 : 4;
+    p.row_tiles = 1;
+    while (p.row_tiles < most && p.row_tiles * 16 < rows) {
+        p.row_tiles *= 2;
+    }
+    p.row_blocks = static_cast<uint32_t>((rows + p.row_tiles * 16 - 1) / (p.row_tiles * 16));
+    const uint32_t tiles = len / attend_tile + (len % attend_tile != 0);
+    const uint32_t splits = attend_max_splits_of(p, n_kv, len);
+    p.chunk = std::max(1u, (tiles + splits - 1) / splits);
+    p.splits = std::max(1u, (tiles + p.chunk - 1) / p.chunk);
+    return p;
+}
+
+// Scratch a plan needs: per split, KV head and query row an output and its
+// (max, sum); none for a single split.
+inline uint64_t attend_scratch_floats(const attend_plan& p, uint32_t n_kv, uint64_t rows, uint32_t hd) {
+    return p.splits > 1 ? uint64_t{p.splits} * n_kv * rows * (hd + 2) : 0;
+}
+
+// The most any call of up to max_n tokens on up to max_len keys needs: splits
+// only grow with the keys, and there are none from some count of rows on.
+inline uint64_t attend_scratch_bound(uint32_t max_n, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t max_len,
+                                     bool eight) {
+    uint64_t most = 0;
+    for (uint32_t n = 1; n <= max_n; ++n) {
+        const attend_plan p = plan_attend_rows(n, group, n_kv, hd, max_len, eight);
+        if (uint64_t{p.row_blocks} * n_kv * 2 > attend_split_blocks) {
+            break;
+        }
+        const uint64_t rows = uint64_t{n} * group;
+        const uint32_t splits = attend_max_splits_of(p, n_kv, max_len);
+        if (splits > 1) {
+            most = std::max(most, splits * n_kv * rows * (hd + 2));
+        }
+    }
+    return most;
+}
+
+}  // namespace syn

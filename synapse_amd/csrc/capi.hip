@@ -13,6 +13,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
@@ -351,6 +352,278 @@ int attend_checked(syn_arena* a, const syn_attn_desc* d, bool with_new_rows, con
         return hip_status(syn::launch_prefill(f, d->q_dtype, a->stream), "prefill launch");
     }
     return hip_status(syn::launch_generic_causal(f, d->q_dtype, a->stream), "generic causal launch");
+}
+
+// ---- 8-bit KV states and drafted trees ---------------------------------------
+
+// The arena's device for as long as it lives: launches go to the current
+// device, which a caller of several GPUs may have changed.
+class on_device {
+public:
+    explicit on_device(int device) {
+        if (hipGetDevice(&was_) == hipSuccess && was_ != device) {
+            changed_ = hipSetDevice(device) == hipSuccess;
+        }
+    }
+    ~on_device() {
+        if (changed_) {
+            (void)hipSetDevice(was_);
+        }
+    }
+    on_device(const on_device&) = delete;
+    on_device& operator=(const on_device&) = delete;
+
+private:
+    int was_ = 0;
+    bool changed_ = false;
+};
+
+constexpr uint32_t rows_max_ctx = 0x7fffffffu - 63;  // tile arithmetic stays in 31 bits
+
+bool kv8_shape_ok(uint32_t max_ctx, uint32_t n_kv, uint32_t hd) {
+    return max_ctx != 0 && max_ctx <= rows_max_ctx && n_kv != 0 && n_kv <= 65536 && hd != 0 && hd <= 256 &&
+           hd % 2 == 0;
+}
+
+struct span {
+    uint64_t at, bytes;
+    const char* what;
+};
+
+// None of `written` may overlap another of them or any of `read` (each
+// already inside the arena).
+int check_apart(const char* call, std::initializer_list<span> written, std::initializer_list<span> read) {
+    for (const span* x = written.begin(); x != written.end(); ++x) {
+        const auto meets = [x](const span& y) {
+            return x->bytes != 0 && y.bytes != 0 && x->at < y.at + y.bytes && y.at < x->at + x->bytes;
+        };
+        for (const span* y = x + 1; y != written.end(); ++y) {
+            if (meets(*y)) {
+                return fail(SYN_HIP_EINVAL, "%s: %s overlaps %s", call, x->what, y->what);
+            }
+        }
+        for (const span& y : read) {
+            if (meets(y)) {
+                return fail(SYN_HIP_EINVAL, "%s: %s overlaps %s", call, x->what, y.what);
+            }
+        }
+    }
+    return SYN_HIP_OK;
+}
+
+int check_kv8(const syn_arena* a, const syn_kv8_desc* c) {
+    if (c == nullptr) {
+        return fail(SYN_HIP_EINVAL, "null cache descriptor");
+    }
+    if (!kv8_shape_ok(c->max_ctx, c->n_kv_heads, c->head_dim)) {
+        return fail(SYN_HIP_EINVAL, "8-bit kv cache: max_ctx %u, n_kv_heads %u, head_dim %u", c->max_ctx,
+                    c->n_kv_heads, c->head_dim);
+    }
+    return check_range(a, c->offset, syn::kv8_bytes(syn::kv8_shape_of(c->max_ctx, c->n_kv_heads, c->head_dim)), 256,
+                       "8-bit kv cache");
+}
+
+span kv8_span(const syn_kv8_desc& c) {
+    return {c.offset, syn::kv8_bytes(syn::kv8_shape_of(c.max_ctx, c.n_kv_heads, c.head_dim)), "the state"};
+}
+
+// Rows pos0..pos0+n-1 of an 8-bit state against row tensors at k and v.
+int check_kv8_rows(const syn_arena* a, const syn_kv8_desc* c, uint64_t k, uint64_t v, uint32_t n, uint32_t pos0,
+                   uint32_t dtype, const char* call, const char* k_what, const char* v_what, uint64_t& bytes) {
+    if (int e = check_arena(a)) {
+        return e;
+    }
+    if (int e = check_kv8(a, c)) {
+        return e;
+    }
+    if (!dtype_ok(dtype)) {
+        return fail(SYN_HIP_EINVAL, "%s: dtype %u", call, dtype);
+    }
+    if (uint64_t{pos0} + n > c->max_ctx) {
+        return fail(SYN_HIP_EINVAL, "%s: %u rows at position %u on a cache of %u", call, n, pos0, c->max_ctx);
+    }
+    bytes = uint64_t{n} * c->n_kv_heads * c->head_dim * dtype_size(dtype);
+    if (int e = check_range(a, k, bytes, dtype_size(dtype), k_what)) {
+        return e;
+    }
+    return check_range(a, v, bytes, dtype_size(dtype), v_what);
+}
+
+syn::kv8_rows_args kv8_rows_of(syn_arena* a, const syn_kv8_desc& c, uint32_t n, uint32_t pos0, uint32_t dtype) {
+    syn::kv8_rows_args r{};
+    r.kv8 = reinterpret_cast<uint8_t*>(a->base + c.offset);
+    r.shape = syn::kv8_shape_of(c.max_ctx, c.n_kv_heads, c.head_dim);
+    r.n = n;
+    r.pos0 = pos0;
+    r.f16 = dtype == SYN_F16;
+    return r;
+}
+
+// A drafted tree's mask (its range and alignment).
+int check_mask(const syn_arena* a, uint64_t offset, uint32_t n, span& at) {
+    const uint64_t bytes = uint64_t{n} * ((uint64_t{n} + 31) / 32) * 4;
+    at = {offset, bytes, "the mask"};
+    return check_range(a, offset, bytes, 4, "tree mask");
+}
+
+// The parts of an attend_rows call that both kinds of state share: the plan,
+// the scratch, and the operands' places.
+int fill_attend_rows(syn_arena* a, syn::attend_rows_args& r, uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t n,
+                     uint32_t pos, float scale, uint32_t q_dtype, uint64_t q_offset, uint64_t out_offset,
+                     uint64_t scratch_offset, uint64_t scratch_bytes, uint64_t mask_offset, bool eight,
+                     std::initializer_list<span> state, const char* call) {
+    const uint32_t group = n_heads / n_kv;
+    const uint64_t rows = uint64_t{n} * group;
+    if (rows > 0x7fffffffu) {
+        return fail(SYN_HIP_EUNSUPPORTED, "%s: %u tokens of %u heads per KV head", call, n, group);
+    }
+    const syn::attend_plan p = syn::plan_attend_rows(n, group, n_kv, hd, pos + n, eight);
+    if (uint64_t{p.row_blocks} * n_kv * p.splits > 0x7fffffffu) {
+        return fail(SYN_HIP_EUNSUPPORTED, "%s: %u tokens of %u heads", call, n, n_heads);
+    }
+    const uint64_t q_bytes = uint64_t{n} * n_heads * hd * dtype_size(q_dtype);
+    const uint64_t out_bytes = uint64_t{n} * n_heads * hd * 4;
+    const uint64_t need = syn::attend_scratch_floats(p, n_kv, rows, hd) * 4;
+    span mask{0, 0, "the mask"};
+    if (mask_offset != no_offset) {
+        if (int e = check_mask(a, mask_offset, n, mask)) {
+            return e;
+        }
+        r.mask = reinterpret_cast<const uint32_t*>(a->base + mask_offset);
+        r.mask_words = n / 32 + (n % 32 != 0);
+    }
+    if (need > scratch_bytes) {
+        return fail(SYN_HIP_EINVAL, "%s: scratch of %llu bytes, %llu needed", call,
+                    static_cast<unsigned long long>(scratch_bytes), static_cast<unsigned long long>(need));
+    }
+    const span out{out_offset, out_bytes, "the output"}, q{q_offset, q_bytes, "q"};
+    span scratch{out_offset, 0, "scratch"};
+    if (need > 0) {
+        if (int e = check_range(a, scratch_offset, need, 16, "attention scratch")) {
+            return e;
+        }
+        scratch = {scratch_offset, need, "scratch"};
+        r.part = reinterpret_cast<float*>(a->base + scratch_offset);
+        r.part_ml = r.part + uint64_t{p.splits} * n_kv * rows * hd;
+    }
+    for (const span& s : state) {
+        if (int e = check_apart(call, {out, scratch}, {q, mask, s})) {
+            return e;
+        }
+    }
+    r.q = a->base + q_offset;
+    r.out = reinterpret_cast<float*>(a->base + out_offset);
+    r.n = n;
+    r.pos = pos;
+    r.n_kv = n_kv;
+    r.group = group;
+    r.hd = hd;
+    r.q_row = n_heads * hd;
+    r.row_tiles = p.row_tiles;
+    r.row_blocks = p.row_blocks;
+    r.chunk = p.chunk;
+    r.splits = p.splits;
+    r.scale_log2e = scale * syn::log2e;
+    r.q_f16 = q_dtype == SYN_F16;
+    return SYN_HIP_OK;
+}
+
+uint64_t attend_rows_scratch(uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t max_ctx, uint32_t max_batch,
+                             bool eight) {
+    if (n_heads == 0 || !kv8_shape_ok(max_ctx, n_kv, hd) || n_heads % n_kv != 0) {
+        return 0;
+    }
+    return align256(syn::attend_scratch_bound(std::min(max_batch, max_ctx), n_heads / n_kv, n_kv, hd, max_ctx, eight) *
+                    4);
+}
+
+int check_kv8_attn(const syn_arena* a, const syn_kv8_attn_desc* d) {
+    if (int e = check_arena(a)) {
+        return e;
+    }
+    if (d == nullptr) {
+        return fail(SYN_HIP_EINVAL, "null descriptor");
+    }
+    if (int e = check_kv8(a, &d->cache)) {
+        return e;
+    }
+    const syn_kv8_desc& c = d->cache;
+    if (d->n_heads == 0 || d->n_heads % c.n_kv_heads != 0) {
+        return fail(SYN_HIP_EINVAL, "kv8 attention: %u query heads on %u KV heads", d->n_heads, c.n_kv_heads);
+    }
+    if (!(std::isfinite(d->scale) && d->scale > 0.0f)) {
+        return fail(SYN_HIP_EINVAL, "kv8 attention: scale %g (want finite and > 0)", static_cast<double>(d->scale));
+    }
+    if (d->n == 0 || uint64_t{d->pos} + d->n > c.max_ctx) {
+        return fail(SYN_HIP_EINVAL, "kv8 attention: run of %u at position %u on a cache of %u", d->n, d->pos,
+                    c.max_ctx);
+    }
+    if (!dtype_ok(d->q_dtype) || !dtype_ok(d->kv_dtype)) {
+        return fail(SYN_HIP_EINVAL, "kv8 attention: dtypes %u, %u", d->q_dtype, d->kv_dtype);
+    }
+    const uint64_t qsize = uint64_t{d->n_heads} * c.head_dim;
+    if (qsize > 0x7fffffffu) {
+        return fail(SYN_HIP_EUNSUPPORTED, "kv8 attention: rows of %llu", static_cast<unsigned long long>(qsize));
+    }
+    if (int e = check_range(a, d->q_offset, d->n * qsize * dtype_size(d->q_dtype), 16, "kv8 attention q")) {
+        return e;
+    }
+    return check_range(a, d->out_offset, d->n * qsize * 4, 16, "kv8 attention out");
+}
+
+// Everything of an attention call on an 8-bit state but its new rows.
+int fill_kv8_attend(syn_arena* a, const syn_kv8_attn_desc* d, syn::attend_rows_args& r) {
+    if (int e = check_kv8_attn(a, d)) {
+        return e;
+    }
+    const syn_kv8_desc& c = d->cache;
+    if (int e = fill_attend_rows(a, r, d->n_heads, c.n_kv_heads, c.head_dim, d->n, d->pos, d->scale, d->q_dtype,
+                                 d->q_offset, d->out_offset, d->scratch_offset, d->scratch_bytes, d->mask_offset,
+                                 true, {kv8_span(c)}, "kv8 attention")) {
+        return e;
+    }
+    const syn::kv8_shape s = syn::kv8_shape_of(c.max_ctx, c.n_kv_heads, c.head_dim);
+    r.kv8 = reinterpret_cast<const uint8_t*>(a->base + c.offset);
+    r.tiles_per_head = s.tiles;
+    r.tile_bytes = s.tile_bytes;
+    r.v_at = s.v_at;
+    r.ks_at = s.ks_at;
+    r.vs_at = s.vs_at;
+    return SYN_HIP_OK;
+}
+
+// The drafted rows a keep call moves; `first` skips those already in place.
+int check_keep(uint32_t pos, uint32_t n, uint32_t max_ctx, const uint32_t* rows, uint32_t count, uint32_t& first) {
+    if (n > 65536 || uint64_t{pos} + n > max_ctx) {
+        return fail(SYN_HIP_EINVAL, "keep: %u drafted rows at position %u on a cache of %u", n, pos, max_ctx);
+    }
+    if (count > n || (count > 0 && rows == nullptr)) {
+        return fail(SYN_HIP_EINVAL, "keep: %u of %u rows%s", count, n, rows == nullptr ? ", null" : "");
+    }
+    first = 0;
+    for (uint32_t i = 0; i < count; ++i) {
+        if (rows[i] >= n || (i > 0 && rows[i] <= rows[i - 1])) {
+            return fail(SYN_HIP_EINVAL, "keep: row %u of %u (want rising rows below %u)", rows[i], i, n);
+        }
+        first += rows[i] == i;
+    }
+    return SYN_HIP_OK;
+}
+
+// Rows first..count in launches of keep_max_rows, front to back.
+template <class LAUNCH>
+int keep_in_launches(const uint32_t* rows, uint32_t first, uint32_t count, LAUNCH launch) {
+    for (; first < count; first += syn::keep_max_rows) {
+        syn::keep_rows part{};
+        const uint32_t m = std::min(count - first, syn::keep_max_rows);
+        for (uint32_t i = 0; i < m; ++i) {
+            part.row[i] = static_cast<uint16_t>(rows[first + i]);
+        }
+        if (int e = hip_status(launch(first, m, part), "keep launch")) {
+            return e;
+        }
+    }
+    return SYN_HIP_OK;
 }
 
 }  // namespace
@@ -1272,6 +1545,152 @@ int syn_hip_pixel_shuffle(syn_arena* a, const syn_pixel_shuffle_desc* d) {
                                                 reinterpret_cast<float*>(a->base + d->out_offset), d->n, d->grid_w,
                                                 d->grid_h, d->scale, a->stream),
                       "pixel_shuffle launch");
+}
+
+uint64_t syn_hip_kv8_state_bytes(uint32_t max_ctx, uint32_t n_kv_heads, uint32_t head_dim) {
+    return kv8_shape_ok(max_ctx, n_kv_heads, head_dim)
+               ? align256(syn::kv8_bytes(syn::kv8_shape_of(max_ctx, n_kv_heads, head_dim)))
+               : 0;
+}
+
+int syn_hip_kv8_append(syn_arena* a, const syn_kv8_desc* cache, uint64_t k_rows, uint64_t v_rows, uint32_t n,
+                       uint32_t pos0, uint32_t kv_dtype) {
+    uint64_t bytes = 0;
+    if (int e = check_kv8_rows(a, cache, k_rows, v_rows, n, pos0, kv_dtype, "kv8_append", "kv8_append k",
+                               "kv8_append v", bytes)) {
+        return e;
+    }
+    if (int e = check_apart("kv8_append", {kv8_span(*cache)}, {{k_rows, bytes, "k"}, {v_rows, bytes, "v"}})) {
+        return e;
+    }
+    if (n == 0) {
+        return SYN_HIP_OK;
+    }
+    syn::kv8_rows_args r = kv8_rows_of(a, *cache, n, pos0, kv_dtype);
+    r.k_in = a->base + k_rows;
+    r.v_in = a->base + v_rows;
+    const on_device current(a->device);
+    return hip_status(syn::launch_kv8_append(r, a->stream), "kv8_append launch");
+}
+
+int syn_hip_kv8_read(syn_arena* a, const syn_kv8_desc* cache, uint64_t k_out, uint64_t v_out, uint32_t n,
+                     uint32_t pos0, uint32_t out_dtype) {
+    uint64_t bytes = 0;
+    if (int e = check_kv8_rows(a, cache, k_out, v_out, n, pos0, out_dtype, "kv8_read", "kv8_read k", "kv8_read v",
+                               bytes)) {
+        return e;
+    }
+    if (int e = check_apart("kv8_read", {{k_out, bytes, "k"}, {v_out, bytes, "v"}}, {kv8_span(*cache)})) {
+        return e;
+    }
+    if (n == 0) {
+        return SYN_HIP_OK;
+    }
+    syn::kv8_rows_args r = kv8_rows_of(a, *cache, n, pos0, out_dtype);
+    r.k_out = a->base + k_out;
+    r.v_out = a->base + v_out;
+    const on_device current(a->device);
+    return hip_status(syn::launch_kv8_read(r, a->stream), "kv8_read launch");
+}
+
+uint64_t syn_hip_kv8_attention_scratch_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                             uint32_t max_ctx, uint32_t max_batch) {
+    return attend_rows_scratch(n_heads, n_kv_heads, head_dim, max_ctx, max_batch, true);
+}
+
+uint64_t syn_hip_attend_tree_scratch_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                           uint32_t max_ctx, uint32_t max_batch) {
+    return attend_rows_scratch(n_heads, n_kv_heads, head_dim, max_ctx, max_batch, false);
+}
+
+int syn_hip_kv8_attend(syn_arena* a, const syn_kv8_attn_desc* d) {
+    syn::attend_rows_args r{};
+    if (int e = fill_kv8_attend(a, d, r)) {
+        return e;
+    }
+    const on_device current(a->device);
+    return hip_status(syn::launch_attend_kv8(r, a->stream), "kv8 attention launch");
+}
+
+int syn_hip_kv8_attention(syn_arena* a, const syn_kv8_attn_desc* d) {
+    syn::attend_rows_args r{};
+    if (int e = fill_kv8_attend(a, d, r)) {  // before the append: a refused call changes nothing
+        return e;
+    }
+    if (int e = syn_hip_kv8_append(a, &d->cache, d->k_offset, d->v_offset, d->n, d->pos, d->kv_dtype)) {
+        return e;
+    }
+    const on_device current(a->device);
+    return hip_status(syn::launch_attend_kv8(r, a->stream), "kv8 attention launch");
+}
+
+int syn_hip_attend_tree(syn_arena* a, const syn_attn_desc* d, uint64_t mask_offset) {
+    if (int e = check_attn(a, d, false)) {
+        return e;
+    }
+    const syn_kv_desc& c = d->cache;
+    if (c.max_ctx > rows_max_ctx || uint64_t{d->n_heads} * c.head_dim > 0x7fffffffu) {
+        return fail(SYN_HIP_EUNSUPPORTED, "attend_tree: max_ctx %u, %u heads", c.max_ctx, d->n_heads);
+    }
+    if (mask_offset == no_offset) {
+        return fail(SYN_HIP_EINVAL, "attend_tree: no mask");
+    }
+    const uint64_t row = uint64_t{c.n_kv_heads} * c.head_dim;
+    syn::attend_rows_args r{};
+    if (int e = fill_attend_rows(a, r, d->n_heads, c.n_kv_heads, c.head_dim, d->n, d->pos, d->scale, d->q_dtype,
+                                 d->q_offset, d->out_offset, d->scratch_offset, d->scratch_bytes, mask_offset, false,
+                                 {{c.k_offset, uint64_t{c.max_ctx} * row * 2, "the state's K"},
+                                  {c.v_offset, row * c.ctx_stride * 2, "the state's V^T"}},
+                                 "attend_tree")) {
+        return e;
+    }
+    r.k = reinterpret_cast<const _Float16*>(a->base + c.k_offset);
+    r.vt = reinterpret_cast<const _Float16*>(a->base + c.v_offset);
+    r.row = c.n_kv_heads * c.head_dim;
+    r.ctx_stride = c.ctx_stride;
+    const on_device current(a->device);
+    return hip_status(syn::launch_attend_tree(r, a->stream), "attend_tree launch");
+}
+
+int syn_hip_kv_keep(syn_arena* a, const syn_kv_desc* cache, uint32_t pos, uint32_t n, const uint32_t* rows,
+                    uint32_t count) {
+    if (int e = check_arena(a)) {
+        return e;
+    }
+    if (cache == nullptr) {
+        return fail(SYN_HIP_EINVAL, "null cache descriptor");
+    }
+    if (int e = check_cache(a, *cache)) {
+        return e;
+    }
+    uint32_t first = 0;
+    if (int e = check_keep(pos, n, cache->max_ctx, rows, count, first)) {
+        return e;
+    }
+    const on_device current(a->device);
+    return keep_in_launches(rows, first, count, [&](uint32_t at, uint32_t m, const syn::keep_rows& part) {
+        return syn::launch_kv_keep(layout_of(a, *cache), pos, at, m, part, a->stream);
+    });
+}
+
+int syn_hip_kv8_keep(syn_arena* a, const syn_kv8_desc* cache, uint32_t pos, uint32_t n, const uint32_t* rows,
+                     uint32_t count) {
+    if (int e = check_arena(a)) {
+        return e;
+    }
+    if (int e = check_kv8(a, cache)) {
+        return e;
+    }
+    uint32_t first = 0;
+    if (int e = check_keep(pos, n, cache->max_ctx, rows, count, first)) {
+        return e;
+    }
+    const syn::kv8_shape s = syn::kv8_shape_of(cache->max_ctx, cache->n_kv_heads, cache->head_dim);
+    const on_device current(a->device);
+    return keep_in_launches(rows, first, count, [&](uint32_t at, uint32_t m, const syn::keep_rows& part) {
+        return syn::launch_kv8_keep(reinterpret_cast<uint8_t*>(a->base + cache->offset), s, pos, at, m, part,
+                                    a->stream);
+    });
 }
 
 }  // extern "C"

@@ -3,6 +3,7 @@
 // C ABI (capi.hip) validates every shape and offset before calling one.
 #pragma once
 
+#include "attend_rows_plan.hpp"
 #include "decode_lds.hpp"
 #include "device.hpp"
 #include "quant_plan.hpp"
@@ -251,6 +252,56 @@ struct flash_args {
 bool prefill_fits(uint32_t kv_len, uint32_t row, uint32_t hd, uint32_t ctx_stride);
 hipError_t launch_prefill(const flash_args& a, uint32_t q_dtype, hipStream_t stream);
 hipError_t launch_bidirectional(const flash_args& a, uint32_t in_dtype, hipStream_t stream);
+
+// ---- 8-bit KV states and drafted trees ---------------------------------------
+// A run's n tokens attend keys 0 .. pos + n - 1 of a KV state (attend_rows.hpp):
+// causally, or with a mask keys 0 .. pos - 1 and the drafted tokens that their
+// row of the mask names.
+struct attend_rows_args {
+    const void* q;           // n rows of q_row, f32 or (q_f16) binary16
+    float* out;              // n rows of q_row
+    float* part;             // split partials: outputs [split][KV head][row][hd]
+    float* part_ml;          //   and their (max, sum)
+    const uint8_t* kv8;      // an 8-bit state's records, or
+    const _Float16* k;       // a binary16 state's K block
+    const _Float16* vt;      //   and V^T block
+    const uint32_t* mask;    // n rows of mask_words words
+    uint32_t mask_words;
+    uint32_t n, pos, n_kv, group, hd, q_row;
+    uint32_t row, ctx_stride;                                // binary16 state
+    uint32_t tiles_per_head, tile_bytes, v_at, ks_at, vs_at; // 8-bit state
+    uint32_t row_tiles, row_blocks, chunk, splits;           // attend_plan
+    float scale_log2e;
+    bool q_f16;
+};
+hipError_t launch_attend_merge(const attend_rows_args& a, hipStream_t stream);
+hipError_t launch_attend_kv8(const attend_rows_args& a, hipStream_t stream);   // a.mask: a tree, nullptr: causal
+hipError_t launch_attend_tree(const attend_rows_args& a, hipStream_t stream);  // binary16 state
+
+// An 8-bit state's rows written, read and moved (kv8.hip).
+struct kv8_rows_args {
+    uint8_t* kv8;
+    kv8_shape shape;
+    const void* k_in;   // append: n rows of n_kv * hd, f32 or binary16
+    const void* v_in;
+    void* k_out;        // read
+    void* v_out;
+    uint32_t n, pos0;
+    bool f16;
+};
+hipError_t launch_kv8_append(const kv8_rows_args& a, hipStream_t stream);
+hipError_t launch_kv8_read(const kv8_rows_args& a, hipStream_t stream);
+
+constexpr uint32_t keep_max_rows = 256;  // rows moved per launch (kernel argument)
+struct keep_rows {
+    uint16_t row[keep_max_rows];
+};
+// Position pos + first + i <- position pos + rows.row[i] for i < count, the
+// rows rising.
+hipError_t launch_kv_keep(const kv_layout& c, uint32_t pos, uint32_t first, uint32_t count, const keep_rows& rows,
+                          hipStream_t stream);
+hipError_t launch_kv8_keep(uint8_t* kv8, const kv8_shape& s, uint32_t pos, uint32_t first, uint32_t count,
+                           const keep_rows& rows, hipStream_t stream);
 
 // ---- any-shape fallback -----------------------------------------------------
 // A plain f32 kernel for shapes the matrix-core kernels do not take
