@@ -7,27 +7,23 @@ namespace syn {
 
 namespace {
 
-template <int DC, int RT>
-hipError_t by_mask(const attend_rows_args& a, hipStream_t stream) {
-    return a.mask != nullptr ? launch_attend_rows_as<DC, RT, attend::kv8_source<DC>, true>(a, stream)
-                             : launch_attend_rows_as<DC, RT, attend::kv8_source<DC>, false>(a, stream);
-}
-
-template <int DC>
+template <int DC, bool TREE>
 hipError_t by_rows(const attend_rows_args& a, hipStream_t stream) {
-    switch (a.row_tiles) {
+    switch (a.wave_tiles) {
+    case 0:
+        return launch_attend_blocks(attend_few_kernel<DC, attend::kv8_source<DC>, TREE>, a, stream);
     case 1:
-        return by_mask<DC, 1>(a, stream);
+        return launch_attend_blocks(attend_many_kernel<DC, 1, true, true, TREE>, a, stream);
     case 2:
-        return by_mask<DC, 2>(a, stream);
-    case 4:
-        if constexpr (DC <= 4) {
-            return by_mask<DC, 4>(a, stream);
-        }
-        [[fallthrough]];
+        return launch_attend_blocks(attend_many_kernel<DC, 2, true, true, TREE>, a, stream);
     default:
         return hipErrorInvalidValue;
     }
+}
+
+template <int DC>
+hipError_t by_mask(const attend_rows_args& a, hipStream_t stream) {
+    return a.mask != nullptr ? by_rows<DC, true>(a, stream) : by_rows<DC, false>(a, stream);
 }
 
 }  // namespace
@@ -35,21 +31,21 @@ hipError_t by_rows(const attend_rows_args& a, hipStream_t stream) {
 hipError_t launch_attend_kv8(const attend_rows_args& a, hipStream_t stream) {
     switch ((a.hd + 31) / 32) {
     case 1:
-        return by_rows<1>(a, stream);
+        return by_mask<1>(a, stream);
     case 2:
-        return by_rows<2>(a, stream);
+        return by_mask<2>(a, stream);
     case 3:
-        return by_rows<3>(a, stream);
+        return by_mask<3>(a, stream);
     case 4:
-        return by_rows<4>(a, stream);
+        return by_mask<4>(a, stream);
     case 5:
-        return by_rows<5>(a, stream);
+        return by_mask<5>(a, stream);
     case 6:
-        return by_rows<6>(a, stream);
+        return by_mask<6>(a, stream);
     case 7:
-        return by_rows<7>(a, stream);
+        return by_mask<7>(a, stream);
     case 8:
-        return by_rows<8>(a, stream);
+        return by_mask<8>(a, stream);
     default:
         return hipErrorInvalidValue;
     }

@@ -65,20 +65,22 @@ inline constexpr uint32_t kv8_v_at(uint32_t key, uint32_t d) {
 }
 
 // ---- blocks of attend_rows --------------------------------------------------
-constexpr uint32_t attend_tile = 64;        // keys of a wave's step
-constexpr uint32_t attend_waves = 4;        // waves of a block; they share out its keys
+constexpr uint32_t attend_tile = 64;        // keys of a step
+constexpr uint32_t attend_waves = 4;        // waves of a block
 constexpr uint32_t attend_max_splits = 256;
 // Splits are added up to this many blocks (256 CUs, two blocks each).
 constexpr uint32_t attend_split_blocks = 512;
 
 struct attend_plan {
-    uint32_t row_tiles;    // 16-row tiles of query rows per block
+    uint32_t wave_tiles;   // 16-row tiles a wave owns; 0: all four waves have the same 16 rows
+    uint32_t block_rows;   // query rows per block
     uint32_t row_blocks;   // blocks over the query rows of one KV head
     uint32_t chunk;        // key tiles per split
     uint32_t splits;
 };
 
-// The most splits a plan of these row blocks may have on up to len keys.
+// The most splits a plan of these row blocks may have on up to len keys:
+// four tiles each at least, one per wave or per staged row block.
 inline uint32_t attend_max_splits_of(const attend_plan& p, uint32_t n_kv, uint32_t len) {
     const uint64_t units = uint64_t{p.row_blocks} * n_kv;
     const uint32_t tiles = len / attend_tile + (len % attend_tile != 0);
@@ -87,19 +89,15 @@ inline uint32_t attend_max_splits_of(const attend_plan& p, uint32_t n_kv, uint32
         {few, std::max(1u, tiles / attend_waves + (tiles % attend_waves != 0)), attend_max_splits}));
 }
 
-// n tokens of `group` query heads per KV head attend up to len keys.
-inline attend_plan plan_attend_rows(uint32_t n, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t len,
-                                    bool eight) {
+// n tokens of `group` query heads per KV head attend up to len keys. by_pairs:
+// a binary16 state whose K rows are off 16 bytes; its tiles go through
+// registers, which 32 rows a wave do not leave.
+inline attend_plan plan_attend_rows(uint32_t n, uint32_t group, uint32_t n_kv, uint32_t len, bool by_pairs) {
     attend_plan p{};
     const uint64_t rows = uint64_t{n} * group;
-    // Rows' operands and outputs are registers: 64 rows fill them at hd 128.
-    // Binary16 K rows off 16 bytes are read by pairs, in 16-row blocks only.
-    const uint32_t most = !eight && hd % 8 != 0 ? 1 : hd > 128 ? 2 : 4;
-    p.row_tiles = 1;
-    while (p.row_tiles < most && p.row_tiles * 16 < rows) {
-        p.row_tiles *= 2;
-    }
-    p.row_blocks = static_cast<uint32_t>((rows + p.row_tiles * 16 - 1) / (p.row_tiles * 16));
+    p.wave_tiles = rows <= 16 ? 0 : rows <= 64 || by_pairs ? 1 : 2;
+    p.block_rows = p.wave_tiles == 0 ? 16 : p.wave_tiles * 16 * attend_waves;
+    p.row_blocks = static_cast<uint32_t>((rows + p.block_rows - 1) / p.block_rows);
     const uint32_t tiles = len / attend_tile + (len % attend_tile != 0);
     const uint32_t splits = attend_max_splits_of(p, n_kv, len);
     p.chunk = std::max(1u, (tiles + splits - 1) / splits);
@@ -116,10 +114,10 @@ inline uint64_t attend_scratch_floats(const attend_plan& p, uint32_t n_kv, uint6
 // The most any call of up to max_n tokens on up to max_len keys needs: splits
 // only grow with the keys, and there are none from some count of rows on.
 inline uint64_t attend_scratch_bound(uint32_t max_n, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t max_len,
-                                     bool eight) {
+                                     bool by_pairs) {
     uint64_t most = 0;
     for (uint32_t n = 1; n <= max_n; ++n) {
-        const attend_plan p = plan_attend_rows(n, group, n_kv, hd, max_len, eight);
+        const attend_plan p = plan_attend_rows(n, group, n_kv, max_len, by_pairs);
         if (uint64_t{p.row_blocks} * n_kv * 2 > attend_split_blocks) {
             break;
         }

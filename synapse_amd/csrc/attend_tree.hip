@@ -6,25 +6,17 @@ namespace syn {
 
 namespace {
 
-template <int DC, int RT>
-hipError_t whole(const attend_rows_args& a, hipStream_t stream) {
-    return launch_attend_rows_as<DC, RT, attend::f16_source<DC, true>, true>(a, stream);
-}
-
-template <int DC>
+// WHOLE8: K rows on 16 bytes; other head sizes load them by pairs.
+template <int DC, bool WHOLE8>
 hipError_t by_rows(const attend_rows_args& a, hipStream_t stream) {
-    if (a.hd % 8 != 0) {  // K rows off 16 bytes: loads by pairs, in 16-row blocks
-        return a.row_tiles == 1 ? launch_attend_rows_as<DC, 1, attend::f16_source<DC, false>, true>(a, stream)
-                                : hipErrorInvalidValue;
-    }
-    switch (a.row_tiles) {
+    switch (a.wave_tiles) {
+    case 0:
+        return launch_attend_blocks(attend_few_kernel<DC, attend::f16_source<DC, WHOLE8>, true>, a, stream);
     case 1:
-        return whole<DC, 1>(a, stream);
+        return launch_attend_blocks(attend_many_kernel<DC, 1, false, WHOLE8, true>, a, stream);
     case 2:
-        return whole<DC, 2>(a, stream);
-    case 4:
-        if constexpr (DC <= 4) {
-            return whole<DC, 4>(a, stream);
+        if constexpr (WHOLE8) {
+            return launch_attend_blocks(attend_many_kernel<DC, 2, false, true, true>, a, stream);
         }
         [[fallthrough]];
     default:
@@ -32,26 +24,31 @@ hipError_t by_rows(const attend_rows_args& a, hipStream_t stream) {
     }
 }
 
+template <int DC>
+hipError_t by_size(const attend_rows_args& a, hipStream_t stream) {
+    return a.hd % 8 == 0 ? by_rows<DC, true>(a, stream) : by_rows<DC, false>(a, stream);
+}
+
 }  // namespace
 
 hipError_t launch_attend_tree(const attend_rows_args& a, hipStream_t stream) {
     switch ((a.hd + 31) / 32) {
     case 1:
-        return by_rows<1>(a, stream);
+        return by_size<1>(a, stream);
     case 2:
-        return by_rows<2>(a, stream);
+        return by_size<2>(a, stream);
     case 3:
-        return by_rows<3>(a, stream);
+        return by_size<3>(a, stream);
     case 4:
-        return by_rows<4>(a, stream);
+        return by_size<4>(a, stream);
     case 5:
-        return by_rows<5>(a, stream);
+        return by_size<5>(a, stream);
     case 6:
-        return by_rows<6>(a, stream);
+        return by_size<6>(a, stream);
     case 7:
-        return by_rows<7>(a, stream);
+        return by_size<7>(a, stream);
     case 8:
-        return by_rows<8>(a, stream);
+        return by_size<8>(a, stream);
     default:
         return hipErrorInvalidValue;
     }

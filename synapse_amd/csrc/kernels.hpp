@@ -270,7 +270,7 @@ struct attend_rows_args {
     uint32_t n, pos, n_kv, group, hd, q_row;
     uint32_t row, ctx_stride;                                // binary16 state
     uint32_t tiles_per_head, tile_bytes, v_at, ks_at, vs_at; // 8-bit state
-    uint32_t row_tiles, row_blocks, chunk, splits;           // attend_plan
+    uint32_t wave_tiles, block_rows, row_blocks, chunk, splits;  // attend_plan
     float scale_log2e;
     bool q_f16;
 };

@@ -41,17 +41,18 @@ int main() {
         const uint32_t group = upto(40), n_kv = upto(64), hd = 2 * upto(128), max_ctx = upto(300000);
         const uint32_t n = upto(max_ctx), max_n = n + upto(100) - 1;
         const uint32_t len = n + (max_ctx > n ? static_cast<uint32_t>(r()) % (max_ctx - n + 1) : 0);
-        const bool eight = i % 2;
-        const syn::attend_plan p = syn::plan_attend_rows(n, group, n_kv, hd, len, eight);
-        CHECK(p.row_tiles == 1 || p.row_tiles == 2 || (p.row_tiles == 4 && hd <= 128));
-        CHECK(eight || hd % 8 == 0 || p.row_tiles == 1);
-        CHECK(uint64_t{p.row_blocks} * p.row_tiles * 16 >= uint64_t{n} * group);
-        CHECK(uint64_t{p.row_blocks - 1} * p.row_tiles * 16 < uint64_t{n} * group);
+        const bool by_pairs = i % 3 == 0;
+        const syn::attend_plan p = syn::plan_attend_rows(n, group, n_kv, len, by_pairs);
+        CHECK(!by_pairs || p.wave_tiles <= 1);
+        CHECK(p.wave_tiles <= 2 && p.block_rows == (p.wave_tiles == 0 ? 16 : 64 * p.wave_tiles));
+        CHECK(p.wave_tiles > 0 || p.row_blocks == 1);
+        CHECK(uint64_t{p.row_blocks} * p.block_rows >= uint64_t{n} * group);
+        CHECK(uint64_t{p.row_blocks - 1} * p.block_rows < uint64_t{n} * group);
         const uint32_t tiles = (len + 63) / 64;
         CHECK(uint64_t{p.chunk} * p.splits >= tiles && uint64_t{p.chunk} * (p.splits - 1) < tiles);
         CHECK(p.splits >= 1 && p.splits <= syn::attend_max_splits);
         CHECK(syn::attend_scratch_floats(p, n_kv, uint64_t{n} * group, hd) <=
-              syn::attend_scratch_bound(std::min(max_n, max_ctx), group, n_kv, hd, max_ctx, eight));
+              syn::attend_scratch_bound(std::min(max_n, max_ctx), group, n_kv, hd, max_ctx, by_pairs));
     }
     CHECK_DONE();
 }
