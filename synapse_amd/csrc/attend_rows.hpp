@@ -40,6 +40,8 @@
 #include "device.hpp"
 #include "kernels.hpp"
 
+#include <type_traits>
+
 namespace syn {
 
 namespace attend {
@@ -47,6 +49,7 @@ namespace attend {
 constexpr float p_shift = 6.0f;  // probabilities are 2^6 exp2(s - m)
 constexpr float lazy = 8.0f;     // a maximum follows once a score is 2^8 above it
 constexpr int no_vexp = -1000;   // no step but zeros so far
+constexpr float no_max = -3.0e38f;  // before any score (finite: a score of -inf is 0, not NaN, over it)
 
 typedef unsigned int u2 __attribute__((ext_vector_type(2)));
 typedef float f2 __attribute__((ext_vector_type(2)));
@@ -60,6 +63,19 @@ __device__ __forceinline__ h8 bytes_h8(unsigned lo, unsigned hi) {
     const h2 c = __builtin_bit_cast(h2, __builtin_amdgcn_perm(one_k, hi, 0x04010400u)) - bias;
     const h2 d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(one_k, hi, 0x04030402u)) - bias;
     return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// x - h[0] and x - h[1], in one instruction each (the compiler converts first
+// and then subtracts).
+__device__ __forceinline__ float less_low(float x, h2 h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
+__device__ __forceinline__ float less_high(float x, h2 h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
 }
 
 __device__ __forceinline__ bool any_lane(bool x) {
@@ -160,7 +176,7 @@ struct wave_rows {
             if constexpr (TREE) {
                 draft[rt] = a.mask + size_t{token} * a.mask_words;
             }
-            mref[rt] = -INFINITY;
+            mref[rt] = no_max;
             l[rt] = 0.0f;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
@@ -227,22 +243,19 @@ struct wave_rows {
         }
     }
 
-    // Scores of the tile at key0 to probabilities, split into hi and lo. ks: the keys' K steps times the scale in exp2's units (or that
-    // scale alone); vm: their V steps over 2^vexp. masked: some row may not
-    // see some of the tile's keys.
-    template <class KS, class VM>
-    __device__ __forceinline__ void softmax(const attend_rows_args& a, const f4 (&s)[RT][4], uint32_t key0, bool masked,
-                                            KS ks, VM vm) {
+    // Scores of the tile at key0 to probabilities, split into hi and lo. ks: the
+    // keys' K steps times the scale in exp2's units (or that scale alone); vm:
+    // their V steps over 2^vexp. MASKED: some row may not see some of the
+    // tile's keys. While no lane has a score more than `lazy` above its row's
+    // maximum, lanes need nothing from each other.
+    template <bool MASKED, class KS, class VM>
+    __device__ __forceinline__ void softmax(const attend_rows_args& a, const f4 (&s)[RT][4], uint32_t key0, KS ks,
+                                            VM vm) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            float p[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                p[j] = s[rt][j / 4][j % 4] * ks(j);
-            }
-            seen[rt] = 0xffffu;
-            if (masked) {
-                uint32_t bits = 0;
+            uint32_t bits = 0xffffu;
+            if constexpr (MASKED) {
+                bits = 0;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const uint32_t k0 = key0 + score_key(8 * c, G);
@@ -255,51 +268,65 @@ struct wave_rows {
                     }
                     bits |= b << (8 * c);
                 }
-                seen[rt] = bits;
+            }
+            seen[rt] = bits;
+            float p[16];  // over the maximum, in exp2's units
+            const auto over = [&](float m) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    p[j] = bits >> j & 1 ? p[j] : -INFINITY;
+                    p[j] = __builtin_fmaf(s[rt][j / 4][j % 4], ks(j), -m);
                 }
-            }
-            float top = p[0];
+                if constexpr (MASKED) {
 #pragma unroll
-            for (int j = 1; j < 16; ++j) {
-                top = fmaxf(top, p[j]);
-            }
-            top = max32(max16(top));
-            const bool follow = top - p_shift > mref[rt] + lazy;
-            if (any_lane(follow)) {
-                const float m = follow ? top - p_shift : mref[rt];
-                const float f = follow ? fast_exp2(mref[rt] - m) : 1.0f;
+                    for (int j = 0; j < 16; ++j) {
+                        p[j] = bits >> j & 1 ? p[j] : -INFINITY;
+                    }
+                }
+                float top = p[0];
+#pragma unroll
+                for (int j = 1; j < 16; ++j) {
+                    top = fmaxf(top, p[j]);
+                }
+                return top;
+            };
+            float top = over(mref[rt]);
+            if (any_lane(top > p_shift + lazy)) {
+                top = max32(max16(over(0.0f))) - p_shift;
+                const float m = top > mref[rt] + lazy ? top : mref[rt];
+                const float f = fast_exp2(mref[rt] - m);
                 mref[rt] = m;
                 l[rt] *= f;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
                     acc[rt][dt] *= f;
                 }
+                over(m);
             }
-            const float m = mref[rt] == -INFINITY ? 0.0f : mref[rt];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                p[j] = fast_exp2(p[j] - m);
+                p[j] = fast_exp2(p[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
                 l[rt] += p[j];
                 if constexpr (EIGHT) {
                     p[j] *= vm(j);
                 }
             }
-            if constexpr (EIGHT) {
-                if (masked) {  // a masked key's step may be NaN
+            if constexpr (EIGHT && MASKED) {  // a masked key's step may be NaN
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        p[j] = seen[rt] >> j & 1 ? p[j] : 0.0f;
-                    }
+                for (int j = 0; j < 16; ++j) {
+                    p[j] = bits >> j & 1 ? p[j] : 0.0f;
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const _Float16 h = to_h(p[j]);
-                hi[rt][j / 8][j % 8] = h;
-                lo[rt][j / 8][j % 8] = to_h(p[j] - static_cast<float>(h));
+            for (int j = 0; j < 16; j += 2) {
+                const h2 h = __builtin_convertvector((f2{p[j], p[j + 1]}), h2);
+                hi[rt][j / 8][j % 8] = h[0];
+                hi[rt][j / 8][j % 8 + 1] = h[1];
+                const h2 r = __builtin_convertvector((f2{less_low(p[j], h), less_high(p[j + 1], h)}), h2);
+                lo[rt][j / 8][j % 8] = r[0];
+                lo[rt][j / 8][j % 8 + 1] = r[1];
             }
         }
     }
@@ -540,7 +567,8 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const attend_rows_args 
     }
     rows.take_q(a, raw);
 
-    while (tile < b.t_end) {
+    const auto step = [&](auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
         f4 s[1][4];
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
@@ -551,13 +579,15 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const attend_rows_args 
             }
         }
         const uint32_t key0 = tile * attend_tile;
-        const bool masked = key0 + attend_tile > open;
         if constexpr (SRC::eight) {
             float vm[16];
             float top = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {  // (past the last key the steps may be anything)
-                vm[j] = key0 + score_key(j, rows.G) < b.len ? src.vs[j / 4][j % 4] : 0.0f;
+            for (int j = 0; j < 16; ++j) {
+                vm[j] = src.vs[j / 4][j % 4];
+                if constexpr (MASKED) {  // past the last key the steps may be anything
+                    vm[j] = key0 + score_key(j, rows.G) < b.len ? vm[j] : 0.0f;
+                }
                 top = fmaxf(top, vm[j]);
             }
             rows.raise_vexp(step_exp(max32(max16(top))));
@@ -565,34 +595,37 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const attend_rows_args 
             for (int j = 0; j < 16; ++j) {
                 vm[j] = ldexpf(vm[j], -rows.vexp);
             }
-            rows.softmax(a, s, key0, masked, [&](int j) { return src.ks[j / 4][j % 4] * a.scale_log2e; },
-                         [&](int j) { return vm[j]; });
+            rows.template softmax<MASKED>(a, s, key0, [&](int j) { return src.ks[j / 4][j % 4] * a.scale_log2e; },
+                                          [&](int j) { return vm[j]; });
         } else {
-            rows.softmax(a, s, key0, masked, [&](int) { return a.scale_log2e; }, [](int) { return 1.0f; });
+            rows.template softmax<MASKED>(a, s, key0, [&](int) { return a.scale_log2e; }, [](int) { return 1.0f; });
         }
-        if (!SRC::eight && masked) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const uint32_t key = key0 + score_key(8 * c, rows.G);
+        for (int c = 0; c < 2; ++c) {
+            const uint32_t key = key0 + score_key(8 * c, rows.G);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
+            for (int dt = 0; dt < DT; ++dt) {
+                if constexpr (!SRC::eight && MASKED) {
                     rows.add_v_tail(dt, c, src.v(dt, c), b.len > key ? b.len - key : 0);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
+                } else {
                     rows.add_v(dt, c, src.v(dt, c));
                 }
             }
         }
-        tile += attend_waves;
-        if (tile < b.t_end) {
-            src.load(tile, lane);
+    };
+    // Tiles that every row sees whole, then the others, in loops of their own:
+    // the masks would take the first one's registers.
+    const auto run = [&](uint32_t to, auto masked) {
+        while (tile < to) {
+            step(masked);
+            tile += attend_waves;
+            if (tile < b.t_end) {
+                src.load(tile, lane);
+            }
         }
-    }
+    };
+    run(min(b.t_end, open / attend_tile), std::false_type{});
+    run(b.t_end, std::true_type{});
 
     // The waves' rows meet in LDS as a weighted mean.
     rows.finish();
@@ -652,8 +685,8 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
     const uint32_t n_rows = a.n * a.group;
     const uint32_t row0 = b.row0 + w * (RT * 16);
     const bool has_rows = row0 < n_rows;
-    // This wave's rows: keys that all of them see, and keys that any sees.
-    const uint32_t open = TREE ? a.pos : a.pos + row0 / a.group + 1;
+    const uint32_t open = TREE ? a.pos : a.pos + b.row0 / a.group + 1;  // keys that all the block's rows see
+    // Keys that any of this wave's rows sees.
     const uint32_t reach = !has_rows ? 0 : TREE ? b.len : a.pos + (min(row0 + RT * 16, n_rows) - 1) / a.group + 1;
 
     const uint8_t* head = EIGHT ? a.kv8 + size_t{b.g} * a.tiles_per_head * a.tile_bytes : nullptr;
@@ -759,74 +792,78 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
     }
     __syncthreads();
     const bool k_in = (DC - 1) * 32 + rows.G * 8 < a.hd;  // the lane's last eight dims are the head's
-    for (uint32_t tile = b.t_begin; tile < b.t_end; ++tile) {
-        const uint32_t buf = (tile - b.t_begin) & 1;
-        const bool more = tile + 1 < b.t_end;
-        if (more) {
-            load(tile + 1, buf ^ 1);
-        }
-        const uint32_t key0 = tile * attend_tile;
-        if (key0 < reach) {
-            const h8* from = &tiles[buf][0][lane];
-            f4 s[RT][4];
+    const auto step = [&](uint32_t key0, uint32_t buf, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        const h8* from = &tiles[buf][0][lane];
+        f4 s[RT][4];
 #pragma unroll
-            for (int st = 0; st < 4; ++st) {
+        for (int st = 0; st < 4; ++st) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                s[rt][st] = f4{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int dc = 0; dc < DC; ++dc) {
+                h8 k = from[(st * DC + dc) * 64];
+                if constexpr (COPY) {
+                    if (dc == DC - 1) {  // (what follows is the next head's, and could be NaN)
+                        k = as_h8(k_in ? as_u4(k) : zero_u4());
+                    }
+                }
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    s[rt][st] = f4{0, 0, 0, 0};
-                }
-#pragma unroll
-                for (int dc = 0; dc < DC; ++dc) {
-                    h8 k = from[(st * DC + dc) * 64];
-                    if constexpr (COPY) {
-                        if (dc == DC - 1) {  // (what follows is the next head's, and could be NaN)
-                            k = as_h8(k_in ? as_u4(k) : zero_u4());
-                        }
-                    }
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        s[rt][st] = mfma16(k, rows.q[rt][dc], s[rt][st]);
-                    }
-                }
-            }
-            const bool masked = key0 + attend_tile > open;
-            if constexpr (EIGHT) {
-                rows.raise_vexp(__builtin_amdgcn_readfirstlane(vexp_lds[buf]));
-                f4 ks[4], vm[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    ks[j] = *reinterpret_cast<const f4*>(&ks_lds[buf][score_key(4 * j, rows.G)]);
-                    vm[j] = *reinterpret_cast<const f4*>(&vs_lds[buf][score_key(4 * j, rows.G)]);
-                }
-                rows.softmax(a, s, key0, masked, [&](int j) { return ks[j / 4][j % 4]; },
-                             [&](int j) { return vm[j / 4][j % 4]; });
-            } else {
-                rows.softmax(a, s, key0, masked, [&](int) { return a.scale_log2e; }, [](int) { return 1.0f; });
-            }
-            if (!EIGHT && masked) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const uint32_t key = key0 + score_key(8 * c, rows.G);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        rows.add_v_tail(dt, c, from[(v_frag + dt * 2 + c) * 64], b.len > key ? b.len - key : 0);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        rows.add_v(dt, c, from[(v_frag + dt * 2 + c) * 64]);
-                    }
+                    s[rt][st] = mfma16(k, rows.q[rt][dc], s[rt][st]);
                 }
             }
         }
-        if (more) {
-            stage(buf ^ 1);
+        if constexpr (EIGHT) {
+            rows.raise_vexp(__builtin_amdgcn_readfirstlane(vexp_lds[buf]));
+            f4 ks[4], vm[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                ks[j] = *reinterpret_cast<const f4*>(&ks_lds[buf][score_key(4 * j, rows.G)]);
+                vm[j] = *reinterpret_cast<const f4*>(&vs_lds[buf][score_key(4 * j, rows.G)]);
+            }
+            rows.template softmax<MASKED>(a, s, key0, [&](int j) { return ks[j / 4][j % 4]; },
+                                          [&](int j) { return vm[j / 4][j % 4]; });
+        } else {
+            rows.template softmax<MASKED>(a, s, key0, [&](int) { return a.scale_log2e; }, [](int) { return 1.0f; });
         }
-        __syncthreads();
-    }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const uint32_t key = key0 + score_key(8 * c, rows.G);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const h8 v = from[(v_frag + dt * 2 + c) * 64];
+                if constexpr (!EIGHT && MASKED) {
+                    rows.add_v_tail(dt, c, v, b.len > key ? b.len - key : 0);
+                } else {
+                    rows.add_v(dt, c, v);
+                }
+            }
+        }
+    };
+    // Tiles that every row of the block sees whole, then the others, in loops
+    // of their own: the masks would take the first one's registers.
+    const auto run = [&](uint32_t from, uint32_t to, auto masked) {
+        for (uint32_t tile = from; tile < to; ++tile) {
+            const uint32_t buf = (tile - b.t_begin) & 1;
+            const bool more = tile + 1 < b.t_end;
+            if (more) {
+                load(tile + 1, buf ^ 1);
+            }
+            if (tile * attend_tile < reach) {
+                step(tile * attend_tile, buf, masked);
+            }
+            if (more) {
+                stage(buf ^ 1);
+            }
+            __syncthreads();
+        }
+    };
+    const uint32_t whole = max(b.t_begin, min(b.t_end, open / attend_tile));
+    run(b.t_begin, whole, std::false_type{});
+    run(whole, b.t_end, std::true_type{});
 
     rows.finish();
 #pragma unroll
