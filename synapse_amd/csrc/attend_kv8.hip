@@ -9,13 +9,18 @@ namespace {
 
 template <int DC, bool TREE>
 hipError_t by_rows(const attend_rows_args& a, hipStream_t stream) {
-    switch (a.wave_tiles) {
-    case 0:
-        return launch_attend_blocks(attend_few_kernel<DC, attend::kv8_source<DC>, TREE>, a, stream);
-    case 1:
-        return launch_attend_blocks(attend_many_kernel<DC, 1, true, true, TREE>, a, stream);
-    case 2:
-        return launch_attend_blocks(attend_many_kernel<DC, 2, true, true, TREE>, a, stream);
+    switch (a.kernel) {
+    case attend_few:
+        return launch_attend_blocks(attend_few_kernel<DC, attend::kv8_source<DC>, TREE>, 256, a, stream);
+    case attend_many16:
+        return launch_attend_blocks(attend_many_kernel<DC, 1, true, true, TREE>, 256, a, stream);
+    case attend_many32:
+        return launch_attend_blocks(attend_many_kernel<DC, 2, true, true, TREE>, 256, a, stream);
+    case attend_turns:
+        if constexpr (DC <= 4) {
+            return launch_attend_blocks(attend_turns_kernel<DC, true, TREE>, 512, a, stream);
+        }
+        [[fallthrough]];
     default:
         return hipErrorInvalidValue;
     }

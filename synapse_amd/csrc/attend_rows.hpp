@@ -141,37 +141,132 @@ __device__ __forceinline__ int step_exp(float top) {
     return __builtin_amdgcn_readfirstlane(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : no_vexp);
 }
 
+// x / group for x below 2^32 / group (a row of the block, counted from its
+// first token's first head).
+__device__ __forceinline__ uint32_t div_group(const attend_rows_args& a, uint32_t x) {
+    return a.group == 1 ? x : __umulhi(x, a.inv_group);
+}
+
+// A block's place: KV heads fastest (with 8 of them each XCD keeps to one,
+// whose L2 then serves all row blocks), then splits, the last row blocks
+// first (a causal run's longest). A grid of three dimensions, and one division
+// for the block's first row: a launch finds its instructions in neither cache
+// (other kernels and the keys have gone through both), and starting with four
+// divisions to fetch took 2 to 12 us.
+struct block_place {
+    uint32_t g, split, row0, len, t_begin, t_end;
+    uint32_t token0, head0;  // of row0
+};
+template <bool TREE>
+__device__ __forceinline__ block_place place_block(const attend_rows_args& a) {
+    block_place b;
+    b.g = blockIdx.x;
+    b.split = blockIdx.y;
+    b.row0 = (a.row_blocks - 1 - blockIdx.z) * a.block_rows;
+    b.token0 = b.row0 / a.group;
+    b.head0 = b.row0 - b.token0 * a.group;
+    const uint32_t rows = a.n * a.group;
+    const uint32_t last = min(a.block_rows, rows - b.row0) - 1;
+    // Up to the last row's last key.
+    b.len = TREE ? a.pos + a.n : a.pos + b.token0 + div_group(a, b.head0 + last) + 1;
+    const uint32_t tiles = (b.len + attend_tile - 1) / attend_tile;
+    b.t_begin = b.split * a.chunk;
+    b.t_end = min(tiles, b.t_begin + a.chunk);
+    return b;
+}
+
+// Where the output of row r of all, at q's place `at`, goes: the output
+// itself, or its split's part.
+__device__ __forceinline__ float* row_out(const attend_rows_args& a, const block_place& b, uint32_t r, size_t at) {
+    return a.splits == 1 ? a.out + at : a.part + ((size_t{b.split} * a.n_kv + b.g) * (a.n * a.group) + r) * a.hd;
+}
+__device__ __forceinline__ void store_part(const attend_rows_args& a, const block_place& b, uint32_t r, float m,
+                                           float l) {
+    *reinterpret_cast<f2*>(a.part_ml + ((size_t{b.split} * a.n_kv + b.g) * (a.n * a.group) + r) * 2) = f2{m, l};
+}
+
+// The order of stream_operands for the scheduler: a pair's products, two
+// reads, and what goes between (vector work and LDS writes).
+template <int AHEAD, int N, int O, class SHAPE>
+__device__ __forceinline__ void sched_pairs() {
+    if constexpr (O < N) {
+        __builtin_amdgcn_sched_group_barrier(0x008, SHAPE::products(O), 0);
+        if constexpr (O + AHEAD < N) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        if constexpr (SHAPE::valu(O) > 0) {
+            __builtin_amdgcn_sched_group_barrier(0x002, SHAPE::valu(O), 0);
+            __builtin_amdgcn_sched_group_barrier(0x200, 2, 0);
+        }
+        sched_pairs<AHEAD, N, O + 2, SHAPE>();
+    }
+}
+
+// N operands from LDS, used in pairs: `AHEAD` reads are in flight before the
+// first use, and each pair's use is followed by two more and by between(o).
+// Left to itself the compiler reads a pair, waits for it, and only then reads
+// the next one, which left the matrix units idle for as long as they worked.
+// SHAPE: the products of the pair at o, the vector work of between(o).
+template <int AHEAD, int N, class SHAPE, class READ, class USE, class BETWEEN>
+__device__ __forceinline__ void stream_operands(READ read, USE use, BETWEEN between) {
+    static_assert(AHEAD % 2 == 0 && N % 2 == 0 && AHEAD <= N);
+    h8 f[AHEAD];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        f[i] = read(i);
+    }
+#pragma unroll
+    for (int o = 0; o < N; o += 2) {
+        const h8 x = f[o % AHEAD], y = f[o % AHEAD + 1];
+        if (o + AHEAD < N) {
+            f[o % AHEAD] = read(o + AHEAD);
+            f[o % AHEAD + 1] = read(o + AHEAD + 1);
+        }
+        use(o, x, y);
+        between(o);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);  // LDS reads
+    sched_pairs<AHEAD, N, 0, SHAPE>();
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // RT tiles of 16 query rows that one wave holds: lane 16 G + col has column
 // col of every tile.
 template <int DC, int RT, bool EIGHT, bool TREE>
 struct wave_rows {
     static constexpr int DT = 2 * DC;
+    static_assert(RT <= 2);
     uint32_t G, col, row0;
+    uint32_t from;              // row0, counted from the first head of the block's first token
     uint32_t limit[RT];         // keys seen without the mask (0: no row)
     const uint32_t* draft[RT];  // the row's mask
     h8 q[RT][DC];
     f4 acc[RT][DT];             // O^T: dims 16 dt + 4 G .. + 3
-    float mref[RT], l[RT];      // the running maximum less p_shift; the sum of this lane's keys
+    // The running maximum less p_shift; the sum of this lane's keys. Vectors:
+    // as arrays the compiler kept them in LDS by work-item, and finding that
+    // place read the dispatch packet in host memory (1 to 13 us of a start).
+    f2 mref, l;
     h8 hi[RT][2], lo[RT][2];    // the last step's probabilities
     uint32_t seen[RT];          // its keys that the row sees, by score
     int vexp;
 
-    // Starts the rows' loads (f32 rows raw, to be rounded by take_q).
     struct raw_q {
         f4 x[RT][DC][2];
     };
-    __device__ __forceinline__ void place(const attend_rows_args& a, uint32_t g, uint32_t first, uint32_t lane,
-                                          raw_q& raw) {
+    // Rows from row `skip` of the block's on.
+    __device__ __forceinline__ void place(const attend_rows_args& a, const block_place& b, uint32_t skip,
+                                          uint32_t lane) {
         G = lane / 16;
         col = lane % 16;
-        row0 = first;
+        row0 = b.row0 + skip;
+        from = b.head0 + skip;
         vexp = no_vexp;
         const uint32_t rows = a.n * a.group;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const uint32_t r = row0 + rt * 16 + col;
-            const bool in = r < rows;
-            const uint32_t token = in ? r / a.group : 0, head = in ? g * a.group + r % a.group : 0;
+            const bool in = row0 + rt * 16 + col < rows;
+            const uint32_t token = in ? b.token0 + div_group(a, from + rt * 16 + col) : 0;
             limit[rt] = !in ? 0 : TREE ? a.pos : a.pos + token + 1;
             if constexpr (TREE) {
                 draft[rt] = a.mask + size_t{token} * a.mask_words;
@@ -182,48 +277,64 @@ struct wave_rows {
             for (int dt = 0; dt < DT; ++dt) {
                 acc[rt][dt] = f4{0, 0, 0, 0};
             }
-            const size_t at = size_t{token} * a.q_row + head * a.hd;
+        }
+    }
+    // A row's place in q and in the output (0: no row).
+    __device__ __forceinline__ size_t at(const attend_rows_args& a, const block_place& b, int rt) const {
+        const uint32_t x = from + rt * 16 + col, later = div_group(a, x);
+        return row0 + rt * 16 + col < a.n * a.group
+                   ? size_t{b.token0 + later} * a.q_row + (b.g * a.group + x - later * a.group) * a.hd
+                   : 0;
+    }
+    // Starts the rows' loads, 32 bytes for eight dims (of which binary16 rows
+    // use the first 16), with no branch on the type: at a join the compiler
+    // waited for what each side had loaded, one operand after the other (8 us
+    // of a block's start). Heads of no whole eights are loaded by take_q.
+    __device__ __forceinline__ void load_q(const attend_rows_args& a, const block_place& b, raw_q& raw) const {
+        if (a.hd % 8 == 0) {
+            const uint32_t size = a.q_f16 ? 2 : 4, half = a.q_f16 ? 0 : 16;
 #pragma unroll
-            for (int dc = 0; dc < DC; ++dc) {
-                const uint32_t d = k_dim<DC, EIGHT>(dc, G);
-                if (a.hd % 8 == 0) {
-                    const size_t i = d < a.hd ? at + d : 0;
-                    if (a.q_f16) {
-                        raw.x[rt][dc][0] = __builtin_bit_cast(f4, load16(static_cast<const _Float16*>(a.q) + i));
-                    } else {
-                        raw.x[rt][dc][0] = *reinterpret_cast<const f4*>(static_cast<const float*>(a.q) + i);
-                        raw.x[rt][dc][1] = *reinterpret_cast<const f4*>(static_cast<const float*>(a.q) + i + 4);
-                    }
-                } else {
-                    h8 x;
+            for (int rt = 0; rt < RT; ++rt) {
+                const size_t i = at(a, b, rt);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const size_t i = d + e < a.hd ? at + d + e : 0;
-                        x[e] = a.q_f16 ? static_cast<const _Float16*>(a.q)[i] : to_h(static_cast<const float*>(a.q)[i]);
-                        x[e] = d + e < a.hd ? x[e] : static_cast<_Float16>(0);
-                    }
-                    raw.x[rt][dc][0] = __builtin_bit_cast(f4, x);
+                for (int dc = 0; dc < DC; ++dc) {
+                    const uint32_t d = k_dim<DC, EIGHT>(dc, G);
+                    const char* p = static_cast<const char*>(a.q) + (i + (d < a.hd ? d : 0)) * size;
+                    raw.x[rt][dc][0] = *reinterpret_cast<const f4*>(p);
+                    raw.x[rt][dc][1] = *reinterpret_cast<const f4*>(p + half);
                 }
             }
         }
     }
-    __device__ __forceinline__ void take_q(const attend_rows_args& a, const raw_q& raw) {
+    // Rounds them to binary16; zeros past the head's last dim.
+    __device__ __forceinline__ void take_q(const attend_rows_args& a, const block_place& b, const raw_q& raw) {
+        if (a.hd % 8 == 0) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                for (int dc = 0; dc < DC; ++dc) {
+                    const f4 x = raw.x[rt][dc][0], y = raw.x[rt][dc][1];
+                    h8 h = a.q_f16 ? __builtin_bit_cast(h8, x)
+                                   : h8{to_h(x[0]), to_h(x[1]), to_h(x[2]), to_h(x[3]), to_h(y[0]), to_h(y[1]),
+                                        to_h(y[2]), to_h(y[3])};
+                    q[rt][dc] = k_dim<DC, EIGHT>(dc, G) < a.hd ? h : as_h8(zero_u4());
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
+            const size_t row = at(a, b, rt);
 #pragma unroll
             for (int dc = 0; dc < DC; ++dc) {
-                const f4 x = raw.x[rt][dc][0], y = raw.x[rt][dc][1];
-                h8 h = __builtin_bit_cast(h8, x);
-                if (a.hd % 8 == 0) {
-                    if (!a.q_f16) {
-                        h = h8{to_h(x[0]), to_h(x[1]), to_h(x[2]), to_h(x[3]), to_h(y[0]), to_h(y[1]), to_h(y[2]),
-                               to_h(y[3])};
-                    }
-                    if (k_dim<DC, EIGHT>(dc, G) >= a.hd) {
-                        h = as_h8(zero_u4());
-                    }
+                const uint32_t d = k_dim<DC, EIGHT>(dc, G);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const size_t i = row + (d + e < a.hd ? d + e : 0);
+                    const _Float16 x = a.q_f16 ? static_cast<const _Float16*>(a.q)[i]
+                                               : to_h(static_cast<const float*>(a.q)[i]);
+                    q[rt][dc][e] = d + e < a.hd ? x : static_cast<_Float16>(0);
                 }
-                q[rt][dc] = h;
             }
         }
     }
@@ -331,6 +442,91 @@ struct wave_rows {
         }
     }
 
+    // The products of a tile, its operands in LDS in lane order: V (dt, c) at
+    // v_from, then K (st, dc) of the next tile at k_from. Operand o of V is dims
+    // o % DT of key half o / DT, of K score tile o % 4 of k-step o / 4: what
+    // neighbouring products add to lies apart.
+    static constexpr int v_ops = 4 * DC, k_ops = 4 * DC;
+    struct v_shape {
+        static constexpr int products(int) { return 4 * RT; }
+        static constexpr int valu(int) { return 0; }
+    };
+    struct k_shape {
+        static constexpr int products(int) { return 2 * RT; }
+        static constexpr int valu(int) { return 0; }
+    };
+    __device__ static __forceinline__ h8 read_v(const h8* v_from, int o) {
+        return v_from[(o % DT * 2 + o / DT) * 64];
+    }
+    __device__ static __forceinline__ h8 read_k(const h8* k_from, int o) {
+        return k_from[(o % 4 * DC + o / 4) * 64];
+    }
+    __device__ __forceinline__ void use_v(int o, h8 x, h8 y) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            acc[rt][o % DT] = mfma16(x, hi[rt][o / DT], acc[rt][o % DT]);
+            acc[rt][o % DT + 1] = mfma16(y, hi[rt][o / DT], acc[rt][o % DT + 1]);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            acc[rt][o % DT] = mfma16(x, lo[rt][o / DT], acc[rt][o % DT]);
+            acc[rt][o % DT + 1] = mfma16(y, lo[rt][o / DT], acc[rt][o % DT + 1]);
+        }
+    }
+    // k_in: the lane's last eight dims are the head's (else a binary16 state's
+    // operand has the next head's there, which could be NaN).
+    __device__ __forceinline__ void use_k(int o, h8 x, h8 y, f4 (&s)[RT][4], bool k_in) const {
+        if (!EIGHT && o / 4 == DC - 1) {
+            x = as_h8(k_in ? as_u4(x) : zero_u4());
+            y = as_h8(k_in ? as_u4(y) : zero_u4());
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const f4 zero = {0, 0, 0, 0};
+            s[rt][o % 4] = mfma16(x, q[rt][o / 4], o < 4 ? zero : s[rt][o % 4]);
+            s[rt][o % 4 + 1] = mfma16(y, q[rt][o / 4], o < 4 ? zero : s[rt][o % 4 + 1]);
+        }
+    }
+    template <int AHEAD>
+    __device__ __forceinline__ void stream_k(const h8* k_from, f4 (&s)[RT][4], bool k_in) {
+        stream_operands<AHEAD, k_ops, k_shape>([&](int o) { return read_k(k_from, o); },
+                                               [&](int o, h8 x, h8 y) { use_k(o, x, y, s, k_in); }, [](int) {});
+    }
+    template <int AHEAD>
+    __device__ __forceinline__ void stream_v(const h8* v_from) {
+        stream_operands<AHEAD, v_ops, v_shape>([&](int o) { return read_v(v_from, o); },
+                                               [&](int o, h8 x, h8 y) { use_v(o, x, y); }, [](int) {});
+    }
+    // Both, with UNITS pieces of other work between: between(i) is two LDS
+    // writes and UNIT_VALU vector instructions.
+    template <int UNITS, int UNIT_VALU>
+    struct vk_shape {
+        static constexpr int unit(int o) {  // of the pair at o, or -1: spread over V's products
+            const int every = v_ops / 2 / (UNITS + 1) * 2;
+            return every > 0 && o % every == 0 && o / every >= 1 && o / every <= UNITS ? o / every - 1 : -1;
+        }
+        static constexpr int products(int o) { return o < v_ops ? 4 * RT : 2 * RT; }
+        static constexpr int valu(int o) { return unit(o) >= 0 ? UNIT_VALU : 0; }
+    };
+    template <int AHEAD, class SHAPE, class BETWEEN>
+    __device__ __forceinline__ void stream_vk(const h8* v_from, const h8* k_from, f4 (&s)[RT][4], bool k_in,
+                                              BETWEEN between) {
+        stream_operands<AHEAD, v_ops + k_ops, SHAPE>(
+            [&](int o) { return o < v_ops ? read_v(v_from, o) : read_k(k_from, o - v_ops); },
+            [&](int o, h8 x, h8 y) {
+                if (o < v_ops) {
+                    use_v(o, x, y);
+                } else {
+                    use_k(o - v_ops, x, y, s, k_in);
+                }
+            },
+            [&](int o) {
+                if (SHAPE::unit(o) >= 0) {
+                    between(SHAPE::unit(o));
+                }
+            });
+    }
+
     // O^T += V^T P^T for 16 dims and 32 keys.
     __device__ __forceinline__ void add_v(int dt, int c, h8 v) {
 #pragma unroll
@@ -384,6 +580,17 @@ struct wave_rows {
         }
     }
 
+    __device__ __forceinline__ void add_tail(const h8* v_from, uint32_t key0, uint32_t len) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const uint32_t key = key0 + score_key(8 * c, G);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                add_v_tail(dt, c, v_from[(dt * 2 + c) * 64], len > key ? len - key : 0);
+            }
+        }
+    }
+
     // Rows as (maximum, sum, output over sum).
     __device__ __forceinline__ void finish() {
 #pragma unroll
@@ -404,40 +611,38 @@ struct wave_rows {
             }
         }
     }
-};
 
-// Where a row's output goes: the output itself, or its split's part.
-__device__ __forceinline__ float* row_out(const attend_rows_args& a, uint32_t g, uint32_t split, uint32_t r) {
-    if (a.splits == 1) {
-        return a.out + size_t{r / a.group} * a.q_row + (g * a.group + r % a.group) * a.hd;
+    // The finished rows to the output, or to their split's part.
+    __device__ __forceinline__ void store(const attend_rows_args& a, const block_place& b) const {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const uint32_t r = row0 + rt * 16 + col;
+            if (r < a.n * a.group) {
+                float* out = row_out(a, b, r, at(a, b, rt));
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const uint32_t d = dt * 16 + G * 4;
+                    const f4 o = acc[rt][dt];
+                    if (a.hd % 4 == 0) {
+                        if (d < a.hd) {
+                            *reinterpret_cast<f4*>(out + d) = o;
+                        }
+                    } else {
+                        if (d < a.hd) {
+                            *reinterpret_cast<f2*>(out + d) = f2{o[0], o[1]};
+                        }
+                        if (d + 2 < a.hd) {
+                            *reinterpret_cast<f2*>(out + d + 2) = f2{o[2], o[3]};
+                        }
+                    }
+                }
+                if (a.splits > 1 && G == 0) {
+                    store_part(a, b, r, mref[rt], l[rt]);
+                }
+            }
+        }
     }
-    return a.part + ((size_t{split} * a.n_kv + g) * (a.n * a.group) + r) * a.hd;
-}
-__device__ __forceinline__ void store_part(const attend_rows_args& a, uint32_t g, uint32_t split, uint32_t r, float m,
-                                           float l) {
-    *reinterpret_cast<f2*>(a.part_ml + ((size_t{split} * a.n_kv + g) * (a.n * a.group) + r) * 2) = f2{m, l};
-}
-
-// A block's place: KV heads fastest (with 8 of them each XCD keeps to one,
-// whose L2 then serves all row blocks), then splits, the last row blocks
-// first (a causal run's longest).
-struct block_place {
-    uint32_t g, split, row0, len, t_begin, t_end;
 };
-template <bool TREE>
-__device__ __forceinline__ block_place place_block(const attend_rows_args& a) {
-    block_place b;
-    b.g = blockIdx.x % a.n_kv;
-    b.split = blockIdx.x / a.n_kv % a.splits;
-    b.row0 = (a.row_blocks - 1 - blockIdx.x / a.n_kv / a.splits) * a.block_rows;
-    const uint32_t rows = a.n * a.group;
-    const uint32_t last = min(b.row0 + a.block_rows, rows) - 1;
-    b.len = TREE ? a.pos + a.n : a.pos + last / a.group + 1;  // up to the last row's last key
-    const uint32_t tiles = (b.len + attend_tile - 1) / attend_tile;
-    b.t_begin = b.split * a.chunk;
-    b.t_end = min(tiles, b.t_begin + a.chunk);
-    return b;
-}
 
 // ---- up to 16 rows: each wave its own tiles, from memory to operands ---------
 template <int DC>
@@ -559,13 +764,14 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const attend_rows_args 
 
     wave_rows<DC, 1, SRC::eight, TREE> rows;
     typename decltype(rows)::raw_q raw;
-    rows.place(a, b.g, 0, lane, raw);
+    rows.place(a, b, 0, lane);
+    rows.load_q(a, b, raw);
     SRC src(a, b.g, b.len);
     uint32_t tile = b.t_begin + w;
     if (tile < b.t_end) {
         src.load(tile, lane);
     }
-    rows.take_q(a, raw);
+    rows.take_q(a, b, raw);
 
     const auto step = [&](auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
@@ -656,9 +862,11 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const attend_rows_args 
             o[1] += wx == 0.0f ? 0.0f : wx * ox[1];
         }
         o *= sum == 0.0f ? 0.0f : 1.0f / sum;
-        *reinterpret_cast<f2*>(row_out(a, b.g, b.split, r) + d) = o;
+        const uint32_t token = div_group(a, r);
+        const size_t at = size_t{token} * a.q_row + (b.g * a.group + r - token * a.group) * a.hd;
+        *reinterpret_cast<f2*>(row_out(a, b, r, at) + d) = o;
         if (a.splits > 1 && d == 0) {
-            store_part(a, b.g, b.split, r, top, sum);
+            store_part(a, b, r, top, sum);
         }
     }
 }
@@ -670,7 +878,6 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const attend_rows_args 
 template <int DC, int RT, bool EIGHT, bool WHOLE8, bool TREE>
 __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const attend_rows_args a) {
     using namespace attend;
-    constexpr int DT = 2 * DC;
     constexpr int KQ = DC / 2;
     constexpr uint32_t v_frag = 4 * DC;          // first V operand
     constexpr bool COPY = !EIGHT && WHOLE8;      // binary16 operands, copied to LDS as they are
@@ -685,9 +892,11 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
     const uint32_t n_rows = a.n * a.group;
     const uint32_t row0 = b.row0 + w * (RT * 16);
     const bool has_rows = row0 < n_rows;
-    const uint32_t open = TREE ? a.pos : a.pos + b.row0 / a.group + 1;  // keys that all the block's rows see
+    const uint32_t open = TREE ? a.pos : a.pos + b.token0 + 1;  // keys that all the block's rows see
     // Keys that any of this wave's rows sees.
-    const uint32_t reach = !has_rows ? 0 : TREE ? b.len : a.pos + (min(row0 + RT * 16, n_rows) - 1) / a.group + 1;
+    const uint32_t reach = !has_rows ? 0
+                           : TREE    ? b.len
+                                     : a.pos + b.token0 + div_group(a, b.head0 + min(w * RT * 16 + RT * 16, n_rows - b.row0) - 1) + 1;
 
     const uint8_t* head = EIGHT ? a.kv8 + size_t{b.g} * a.tiles_per_head * a.tile_bytes : nullptr;
     const _Float16* kh = EIGHT ? nullptr : a.k + size_t{b.g} * a.hd;
@@ -705,11 +914,8 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
                 next[i] = load16(t + (i * 256 + threadIdx.x) * 16);
             }
             if (w == 0) {
-                const bool in = tile * attend_tile + lane < b.len;  // past the last key the steps may be anything
-                const float x = *reinterpret_cast<const float*>(t + a.ks_at + lane * 4);
-                const float y = *reinterpret_cast<const float*>(t + a.vs_at + lane * 4);
-                next_ks = in ? x : 0.0f;
-                next_vs = in ? y : 0.0f;
+                next_ks = *reinterpret_cast<const float*>(t + a.ks_at + lane * 4);
+                next_vs = *reinterpret_cast<const float*>(t + a.vs_at + lane * 4);
             }
         } else {
             const uint32_t G = lane / 16, m = lane % 16;
@@ -738,7 +944,7 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
         }
     };
     // What load started, to buffer buf (and waited for).
-    const auto stage = [&](uint32_t buf) {
+    const auto stage = [&](uint32_t tile, uint32_t buf) {
         h8* to = &tiles[buf][0][0];
         if constexpr (COPY) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -769,6 +975,9 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
                 to[at + then] = bytes_h8(next[i][2], next[i][3]);
             }
             if (w == 0) {
+                const bool in = tile * attend_tile + lane < b.len;  // past the last key the steps may be anything
+                next_ks = in ? next_ks : 0.0f;
+                next_vs = in ? next_vs : 0.0f;
                 const int e = step_exp(wave_reduce_max(next_vs));
                 run_vexp = e > run_vexp ? e : run_vexp;
                 ks_lds[buf][lane] = next_ks * a.scale_log2e;
@@ -783,39 +992,21 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
     wave_rows<DC, RT, EIGHT, TREE> rows;
     {
         typename decltype(rows)::raw_q raw;
-        rows.place(a, b.g, row0, lane, raw);
+        rows.place(a, b, w * (RT * 16), lane);
+        rows.load_q(a, b, raw);
         if (b.t_begin < b.t_end) {
             load(b.t_begin, 0);
-            stage(0);
+            stage(b.t_begin, 0);
         }
-        rows.take_q(a, raw);
+        rows.take_q(a, b, raw);
     }
     __syncthreads();
-    const bool k_in = (DC - 1) * 32 + rows.G * 8 < a.hd;  // the lane's last eight dims are the head's
+    const bool k_in = !COPY || (DC - 1) * 32 + rows.G * 8 < a.hd;
     const auto step = [&](uint32_t key0, uint32_t buf, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
         const h8* from = &tiles[buf][0][lane];
         f4 s[RT][4];
-#pragma unroll
-        for (int st = 0; st < 4; ++st) {
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                s[rt][st] = f4{0, 0, 0, 0};
-            }
-#pragma unroll
-            for (int dc = 0; dc < DC; ++dc) {
-                h8 k = from[(st * DC + dc) * 64];
-                if constexpr (COPY) {
-                    if (dc == DC - 1) {  // (what follows is the next head's, and could be NaN)
-                        k = as_h8(k_in ? as_u4(k) : zero_u4());
-                    }
-                }
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    s[rt][st] = mfma16(k, rows.q[rt][dc], s[rt][st]);
-                }
-            }
-        }
+        rows.template stream_k<4>(from, s, k_in);
         if constexpr (EIGHT) {
             rows.raise_vexp(__builtin_amdgcn_readfirstlane(vexp_lds[buf]));
             f4 ks[4], vm[4];
@@ -829,18 +1020,10 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
         } else {
             rows.template softmax<MASKED>(a, s, key0, [&](int) { return a.scale_log2e; }, [](int) { return 1.0f; });
         }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const uint32_t key = key0 + score_key(8 * c, rows.G);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const h8 v = from[(v_frag + dt * 2 + c) * 64];
-                if constexpr (!EIGHT && MASKED) {
-                    rows.add_v_tail(dt, c, v, b.len > key ? b.len - key : 0);
-                } else {
-                    rows.add_v(dt, c, v);
-                }
-            }
+        if constexpr (!EIGHT && MASKED) {
+            rows.add_tail(from + v_frag * 64, key0, b.len);
+        } else {
+            rows.template stream_v<4>(from + v_frag * 64);
         }
     };
     // Tiles that every row of the block sees whole, then the others, in loops
@@ -856,7 +1039,7 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
                 step(tile * attend_tile, buf, masked);
             }
             if (more) {
-                stage(buf ^ 1);
+                stage(tile + 1, buf ^ 1);
             }
             __syncthreads();
         }
@@ -866,42 +1049,262 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
     run(whole, b.t_end, std::true_type{});
 
     rows.finish();
+    rows.store(a, b);
+}
+
+// ---- many rows: two groups of waves that take turns -----------------------------
+// Eight waves of 32 rows; waves w and w + 4 share a SIMD. Between two barriers
+// one group is in its matrix products (P V of a tile and K Q of the next),
+// bringing tiles on the side, the other in its exponentials, so that a SIMD's
+// matrix and vector units work at the same time; waves left to themselves
+// were found in the same phase (matrix units 39 % busy, vector units 47 %, and
+// hardly ever both). In interval 2 i group 0 takes the softmax of tile i, in
+// 2 i + 1 its products; group 1 is one interval behind. The products of tile i
+// read V(i) and K(i + 1), in buffers of their parity, in intervals 2 i + 1 and
+// 2 i + 2. With the products of tile i, group 0 brings K(i + 2), in 2 i + 1,
+// and group 1 V(i + 1), in 2 i + 2: each after the last read of what was there
+// (K(i) in 2 i, V(i - 1) in 2 i) and before the first of what comes (2 i + 3).
+// Group 1 also brings an 8-bit tile's steps(i + 2), in 2 i + 2; a group reads
+// steps(i + 1) into registers at the end of its products of tile i, in 2 i + 1
+// and 2 i + 2, those of i being in registers by 2 i.
+template <int DC, bool EIGHT, bool TREE>
+__global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_args a) {
+    using namespace attend;
+    constexpr int RT = 2, KQ = DC / 2;
+    constexpr int LOADS = (DC + 1) / 2;  // 16-byte units of an 8-bit tile's K or V per thread of a group
+    typedef wave_rows<DC, RT, EIGHT, TREE> wave_rows_t;
+    __shared__ h8 k_lds[2][4 * DC][64], v_lds[2][4 * DC][64];
+    __shared__ float ks_lds[2][attend_tile], vs_lds[2][attend_tile];
+    __shared__ int vexp_lds[2];
+
+    const uint32_t lane = threadIdx.x % 64, in_group = threadIdx.x % 256;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const bool k_group = w < 4;               // group 0: brings K
+    const uint32_t ahead = k_group ? 2 : 1;   // tiles ahead of its products
+    const block_place b = place_block<TREE>(a);
+    const uint32_t n_rows = a.n * a.group;
+    const uint32_t row0 = b.row0 + w * (RT * 16);
+    const uint32_t open = TREE ? a.pos : a.pos + b.token0 + 1;  // keys that all the block's rows see
+    // Keys that any of this wave's rows sees.
+    const uint32_t reach = row0 >= n_rows ? 0
+                           : TREE         ? b.len
+                                          : a.pos + b.token0 + div_group(a, b.head0 + min(w * RT * 16 + RT * 16, n_rows - b.row0) - 1) + 1;
+
+    const uint8_t* head = EIGHT ? a.kv8 + size_t{b.g} * a.tiles_per_head * a.tile_bytes : nullptr;
+    const _Float16* kh = EIGHT ? nullptr : a.k + size_t{b.g} * a.hd;
+    const _Float16* vh = EIGHT ? nullptr : a.vt + size_t{b.g} * a.hd * a.ctx_stride;
+    u4 next[LOADS];
+    float next_ks = 0.0f, next_vs = 0.0f;
+    int run_vexp = no_vexp;  // wave 4's: the steps' power of two up to the staged tile
+
+    // This group's part (K or V) of a tile: 8-bit loads into registers, to be
+    // staged; binary16 copies straight to their buffer. Wave 4 loads the steps
+    // one tile further on.
+    const auto load = [&](uint32_t tile) {
+        if constexpr (EIGHT) {
+            const uint8_t* t = head + size_t{tile} * a.tile_bytes + (k_group ? 0 : a.v_at);
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const uint32_t r = row0 + rt * 16 + rows.col;
-        if (r < n_rows) {
-            float* out = row_out(a, b.g, b.split, r);
+            for (int i = 0; i < LOADS; ++i) {
+                const uint32_t u = i * 256 + in_group;
+                next[i] = load16(t + (DC % 2 == 0 || u < 128 * DC ? u : 0) * 16);
+            }
+        } else {
+            const uint32_t w4 = w % 4, G = lane / 16, m = lane % 16;
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const uint32_t d = dt * 16 + rows.G * 4;
-                const f4 o = rows.acc[rt][dt];
-                if (a.hd % 4 == 0) {
-                    if (d < a.hd) {
-                        *reinterpret_cast<f4*>(out + d) = o;
-                    }
+            for (int i = 0; i < DC; ++i) {
+                const uint32_t f = i * 4 + w4;
+                if (k_group) {
+                    const uint32_t key = tile * attend_tile + operand_key(f / DC, m), d = f % DC * 32 + G * 8;
+                    load16_lds(kh + size_t{key < b.len ? key : b.len - 1} * a.row + (d < a.hd ? d : 0),
+                               &k_lds[tile & 1][f][0]);
                 } else {
-                    if (d < a.hd) {
-                        *reinterpret_cast<f2*>(out + d) = f2{o[0], o[1]};
-                    }
-                    if (d + 2 < a.hd) {
-                        *reinterpret_cast<f2*>(out + d + 2) = f2{o[2], o[3]};
-                    }
+                    const uint32_t d = f / 2 * 16 + m, key = tile * attend_tile + f % 2 * 32 + G * 8;
+                    load16_lds(vh + size_t{d < a.hd ? d : a.hd - 1} * a.ctx_stride + (key < a.ctx_stride ? key : 0),
+                               &v_lds[tile & 1][f][0]);
                 }
             }
-            if (a.splits > 1 && rows.G == 0) {
-                store_part(a, b.g, b.split, r, rows.mref[rt], rows.l[rt]);
+        }
+    };
+    const auto stage_unit = [&](uint32_t tile, int i) {
+        h8* to = k_group ? &k_lds[tile & 1][0][0] : &v_lds[tile & 1][0][0];
+        const uint32_t u = i * 256 + in_group;
+        uint32_t at = u / 64 * 128 + u % 64, then = 64;  // V, and K of whole 64s of dims
+        if (DC % 2 != 0 && k_group) {
+            const uint32_t st = u / (32 * DC), rest = u % (32 * DC);
+            if (rest < 64 * KQ) {
+                at = (st * DC + rest / 64 * 2) * 64 + rest % 64;
+            } else {  // an odd last 32: 8 dims of two keys
+                at = (st * DC + DC - 1) * 64 + (rest - 64 * KQ) * 2;
+                then = 1;
             }
         }
+        if (DC % 2 == 0 || u < 128 * DC) {
+            to[at] = bytes_h8(next[i][0], next[i][1]);
+            to[at + then] = bytes_h8(next[i][2], next[i][3]);
+        }
+    };
+    const auto load_steps = [&](uint32_t tile) {
+        if (EIGHT && w == 4 && tile < b.t_end) {
+            const uint8_t* t = head + size_t{tile} * a.tile_bytes;
+            next_ks = *reinterpret_cast<const float*>(t + a.ks_at + lane * 4);
+            next_vs = *reinterpret_cast<const float*>(t + a.vs_at + lane * 4);
+        }
+    };
+    const auto stage_steps = [&](uint32_t tile) {
+        if (EIGHT && w == 4 && tile < b.t_end) {
+            const bool in = tile * attend_tile + lane < b.len;  // past the last key the steps may be anything
+            const float ks = in ? next_ks : 0.0f, vs = in ? next_vs : 0.0f;
+            const int e = step_exp(wave_reduce_max(vs));
+            run_vexp = e > run_vexp ? e : run_vexp;
+            ks_lds[tile & 1][lane] = ks * a.scale_log2e;
+            vs_lds[tile & 1][lane] = ldexpf(vs, -run_vexp);
+            if (lane == 0) {
+                vexp_lds[tile & 1] = run_vexp;
+            }
+        }
+    };
+    const auto turn = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        lds_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    wave_rows_t rows;
+    rows.place(a, b, w * (RT * 16), lane);
+    f4 s[RT][4];
+    f4 ks[4], vm[4];  // the steps of this lane's keys in the next softmax's tile
+    int vexp = no_vexp;
+    const auto read_steps = [&](uint32_t tile) {
+        if constexpr (EIGHT) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                ks[j] = *reinterpret_cast<const f4*>(&ks_lds[tile & 1][score_key(4 * j, rows.G)]);
+                vm[j] = *reinterpret_cast<const f4*>(&vs_lds[tile & 1][score_key(4 * j, rows.G)]);
+            }
+            vexp = vexp_lds[tile & 1];
+        }
+    };
+    const bool k_in = (DC - 1) * 32 + lane / 16 * 8 < a.hd;
+    const uint32_t t0 = b.t_begin, t1 = b.t_end;
+    if (t0 < t1) {  // (a split of a causal run may lie behind all keys of these rows)
+        // Before the turns: K of the first two tiles, V of the first, steps of
+        // both; the first scores; the loads that the first products stage.
+        typename wave_rows_t::raw_q raw;
+        rows.load_q(a, b, raw);
+        load(t0);
+        load_steps(t0);
+        if constexpr (EIGHT) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                stage_unit(t0, i);
+            }
+            stage_steps(t0);
+            load_steps(t0 + 1);
+        }
+        if (k_group && t0 + 1 < t1) {
+            load(t0 + 1);
+            if constexpr (EIGHT) {
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    stage_unit(t0 + 1, i);
+                }
+            }
+        }
+        if constexpr (EIGHT) {
+            stage_steps(t0 + 1);
+            if (t0 + ahead < t1) {
+                load(t0 + ahead);
+            }
+            load_steps(t0 + 2);
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        rows.take_q(a, b, raw);
+        turn();
+        read_steps(t0);
+        if (t0 * attend_tile < reach) {
+            rows.template stream_k<4>(&k_lds[t0 & 1][0][lane], s, k_in);
+        }
+        turn();
+        if (!k_group) {
+            turn();
+        }
+        const auto run = [&](uint32_t from, uint32_t to, auto masked) {
+            constexpr bool MASKED = decltype(masked)::value;
+            for (uint32_t tile = from; tile < to; ++tile) {
+                const uint32_t key0 = tile * attend_tile;
+                if (key0 < reach) {
+                    if constexpr (EIGHT) {
+                        rows.raise_vexp(__builtin_amdgcn_readfirstlane(vexp));
+                        rows.template softmax<MASKED>(a, s, key0, [&](int j) { return ks[j / 4][j % 4]; },
+                                                      [&](int j) { return vm[j / 4][j % 4]; });
+                    } else {
+                        rows.template softmax<MASKED>(a, s, key0, [&](int) { return a.scale_log2e; },
+                                                      [](int) { return 1.0f; });
+                    }
+                }
+                turn();
+                __builtin_amdgcn_s_setprio(1);
+                const uint32_t bring = tile + ahead;
+                if (!EIGHT && bring < t1) {
+                    load(bring);
+                }
+                // (The last tiles stage what is not read, and behind the last
+                // one the scores are not used: one path for every tile.)
+                const h8* v_from = &v_lds[tile & 1][0][lane];
+                const h8* k_from = &k_lds[(tile + 1) & 1][0][lane];
+                if constexpr (!EIGHT && MASKED) {
+                    if (key0 < reach) {
+                        rows.add_tail(v_from, key0, b.len);
+                        rows.template stream_k<4>(k_from, s, k_in);
+                    }
+                } else if (key0 < reach) {
+                    typedef typename wave_rows_t::template vk_shape<EIGHT && DC % 2 == 0 ? LOADS : 0, 16> shape;
+                    rows.template stream_vk<6, shape>(v_from, k_from, s, k_in,
+                                                      [&](int i) { stage_unit(bring, i); });
+                    if constexpr (EIGHT && DC % 2 != 0) {
+#pragma unroll
+                        for (int i = 0; i < LOADS; ++i) {
+                            stage_unit(bring, i);
+                        }
+                    }
+                } else if constexpr (EIGHT) {
+#pragma unroll
+                    for (int i = 0; i < LOADS; ++i) {
+                        stage_unit(bring, i);
+                    }
+                }
+                if constexpr (EIGHT) {
+                    stage_steps(tile + 2);
+                    if (bring + 1 < t1) {
+                        load(bring + 1);
+                    }
+                    load_steps(tile + 3);
+                    read_steps(tile + 1);
+                } else {
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                }
+                __builtin_amdgcn_s_setprio(0);
+                turn();
+            }
+        };
+        const uint32_t whole = max(t0, min(t1, open / attend_tile));
+        run(t0, whole, std::false_type{});
+        run(whole, t1, std::true_type{});
+        if (k_group) {
+            turn();
+        }
     }
+    rows.finish();
+    rows.store(a, b);
 }
 
 template <class KERNEL>
-hipError_t launch_attend_blocks(KERNEL kernel, const attend_rows_args& a, hipStream_t stream) {
-    const uint64_t blocks = uint64_t{a.row_blocks} * a.n_kv * a.splits;
-    if (blocks > 0x7fffffffu) {
+hipError_t launch_attend_blocks(KERNEL kernel, uint32_t threads, const attend_rows_args& a, hipStream_t stream) {
+    if (a.row_blocks > attend_max_row_blocks || a.group > attend_max_group) {
         return hipErrorInvalidValue;
     }
-    kernel<<<static_cast<uint32_t>(blocks), 256, 0, stream>>>(a);
+    kernel<<<dim3(a.n_kv, a.splits, a.row_blocks), threads, 0, stream>>>(a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess || a.splits == 1) {
         return e;
     }

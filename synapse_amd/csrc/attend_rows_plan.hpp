@@ -68,11 +68,21 @@ inline constexpr uint32_t kv8_v_at(uint32_t key, uint32_t d) {
 constexpr uint32_t attend_tile = 64;        // keys of a step
 constexpr uint32_t attend_waves = 4;        // waves of a block
 constexpr uint32_t attend_max_splits = 256;
-// Splits are added up to this many blocks (256 CUs, two blocks each).
-constexpr uint32_t attend_split_blocks = 512;
+// Splits are added up to this many waves: two on each of 256 CUs' four SIMDs.
+constexpr uint32_t attend_split_waves = 2048;
+
+enum attend_kernel : uint32_t {
+    attend_few,     // one block has the rows, its waves share out the keys
+    attend_many16,  // four waves of 16 rows
+    attend_many32,  // four waves of 32 rows
+    attend_turns,   // eight waves of 32 rows, half of them in their products at a time
+};
+
+constexpr uint32_t attend_max_group = 32768;       // a block's rows of one token more times it stay below 2^32
+constexpr uint32_t attend_max_row_blocks = 65535;  // a grid dimension
 
 struct attend_plan {
-    uint32_t wave_tiles;   // 16-row tiles a wave owns; 0: all four waves have the same 16 rows
+    attend_kernel kernel;
     uint32_t block_rows;   // query rows per block
     uint32_t row_blocks;   // blocks over the query rows of one KV head
     uint32_t chunk;        // key tiles per split
@@ -84,7 +94,8 @@ struct attend_plan {
 inline uint32_t attend_max_splits_of(const attend_plan& p, uint32_t n_kv, uint32_t len) {
     const uint64_t units = uint64_t{p.row_blocks} * n_kv;
     const uint32_t tiles = len / attend_tile + (len % attend_tile != 0);
-    const uint64_t few = units < attend_split_blocks ? attend_split_blocks / units : 1;
+    const uint32_t blocks = attend_split_waves / (p.kernel == attend_turns ? 8 : 4);
+    const uint64_t few = units < blocks ? blocks / units : 1;
     return static_cast<uint32_t>(std::min<uint64_t>(
         {few, std::max(1u, tiles / attend_waves + (tiles % attend_waves != 0)), attend_max_splits}));
 }
@@ -92,11 +103,23 @@ inline uint32_t attend_max_splits_of(const attend_plan& p, uint32_t n_kv, uint32
 // n tokens of `group` query heads per KV head attend up to len keys. by_pairs:
 // a binary16 state whose K rows are off 16 bytes; its tiles go through
 // registers, which 32 rows a wave do not leave.
-inline attend_plan plan_attend_rows(uint32_t n, uint32_t group, uint32_t n_kv, uint32_t len, bool by_pairs) {
+inline attend_plan plan_attend_rows(uint32_t n, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t len,
+                                    bool by_pairs) {
     attend_plan p{};
     const uint64_t rows = uint64_t{n} * group;
-    p.wave_tiles = rows <= 16 ? 0 : rows <= 64 || by_pairs ? 1 : 2;
-    p.block_rows = p.wave_tiles == 0 ? 16 : p.wave_tiles * 16 * attend_waves;
+    if (rows <= 16) {
+        p.kernel = attend_few;
+        p.block_rows = 16;
+    } else if (rows <= 64 || by_pairs) {
+        p.kernel = attend_many16;
+        p.block_rows = 64;
+    } else if (rows <= 128 || hd > 128) {  // over 128 dims a wave's rows leave no second wave on a SIMD
+        p.kernel = attend_many32;
+        p.block_rows = 128;
+    } else {
+        p.kernel = attend_turns;
+        p.block_rows = 256;
+    }
     p.row_blocks = static_cast<uint32_t>((rows + p.block_rows - 1) / p.block_rows);
     const uint32_t tiles = len / attend_tile + (len % attend_tile != 0);
     const uint32_t splits = attend_max_splits_of(p, n_kv, len);
@@ -117,11 +140,11 @@ inline uint64_t attend_scratch_bound(uint32_t max_n, uint32_t group, uint32_t n_
                                      bool by_pairs) {
     uint64_t most = 0;
     for (uint32_t n = 1; n <= max_n; ++n) {
-        const attend_plan p = plan_attend_rows(n, group, n_kv, max_len, by_pairs);
-        if (uint64_t{p.row_blocks} * n_kv * 2 > attend_split_blocks) {
+        const attend_plan p = plan_attend_rows(n, group, n_kv, hd, max_len, by_pairs);
+        const uint64_t rows = uint64_t{n} * group;
+        if (rows * n_kv > attend_split_waves * 64) {  // a wave's most rows: no splits from here on
             break;
         }
-        const uint64_t rows = uint64_t{n} * group;
         const uint32_t splits = attend_max_splits_of(p, n_kv, max_len);
         if (splits > 1) {
             most = std::max(most, splits * n_kv * rows * (hd + 2));

@@ -9,14 +9,19 @@ namespace {
 // WHOLE8: K rows on 16 bytes; other head sizes load them by pairs.
 template <int DC, bool WHOLE8>
 hipError_t by_rows(const attend_rows_args& a, hipStream_t stream) {
-    switch (a.wave_tiles) {
-    case 0:
-        return launch_attend_blocks(attend_few_kernel<DC, attend::f16_source<DC, WHOLE8>, true>, a, stream);
-    case 1:
-        return launch_attend_blocks(attend_many_kernel<DC, 1, false, WHOLE8, true>, a, stream);
-    case 2:
+    switch (a.kernel) {
+    case attend_few:
+        return launch_attend_blocks(attend_few_kernel<DC, attend::f16_source<DC, WHOLE8>, true>, 256, a, stream);
+    case attend_many16:
+        return launch_attend_blocks(attend_many_kernel<DC, 1, false, WHOLE8, true>, 256, a, stream);
+    case attend_many32:
         if constexpr (WHOLE8) {
-            return launch_attend_blocks(attend_many_kernel<DC, 2, false, true, true>, a, stream);
+            return launch_attend_blocks(attend_many_kernel<DC, 2, false, true, true>, 256, a, stream);
+        }
+        return hipErrorInvalidValue;
+    case attend_turns:
+        if constexpr (WHOLE8 && DC <= 4) {
+            return launch_attend_blocks(attend_turns_kernel<DC, false, true>, 512, a, stream);
         }
         [[fallthrough]];
     default:

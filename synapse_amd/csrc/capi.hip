@@ -477,9 +477,9 @@ int fill_attend_rows(syn_arena* a, syn::attend_rows_args& r, uint32_t n_heads, u
     if (rows > 0x7fffffffu) {
         return fail(SYN_HIP_EUNSUPPORTED, "%s: %u tokens of %u heads per KV head", call, n, group);
     }
-    const syn::attend_plan p = syn::plan_attend_rows(n, group, n_kv, pos + n, by_pairs);
-    if (uint64_t{p.row_blocks} * n_kv * p.splits > 0x7fffffffu) {
-        return fail(SYN_HIP_EUNSUPPORTED, "%s: %u tokens of %u heads", call, n, n_heads);
+    const syn::attend_plan p = syn::plan_attend_rows(n, group, n_kv, hd, pos + n, by_pairs);
+    if (p.row_blocks > syn::attend_max_row_blocks || group > syn::attend_max_group) {
+        return fail(SYN_HIP_EUNSUPPORTED, "%s: %u tokens of %u heads per KV head", call, n, group);
     }
     const uint64_t q_bytes = uint64_t{n} * n_heads * hd * dtype_size(q_dtype);
     const uint64_t out_bytes = uint64_t{n} * n_heads * hd * 4;
@@ -517,9 +517,10 @@ int fill_attend_rows(syn_arena* a, syn::attend_rows_args& r, uint32_t n_heads, u
     r.pos = pos;
     r.n_kv = n_kv;
     r.group = group;
+    r.inv_group = static_cast<uint32_t>(((uint64_t{1} << 32) + group - 1) / group);  // (group 1 has no use for it)
     r.hd = hd;
     r.q_row = n_heads * hd;
-    r.wave_tiles = p.wave_tiles;
+    r.kernel = p.kernel;
     r.block_rows = p.block_rows;
     r.row_blocks = p.row_blocks;
     r.chunk = p.chunk;
@@ -1630,7 +1631,7 @@ int syn_hip_attend_tree(syn_arena* a, const syn_attn_desc* d, uint64_t mask_offs
         return e;
     }
     const syn_kv_desc& c = d->cache;
-    if (c.max_ctx > rows_max_ctx || uint64_t{d->n_heads} * c.head_dim > 0x7fffffffu) {
+    if (c.max_ctx > rows_max_ctx || c.n_kv_heads > 65536 || uint64_t{d->n_heads} * c.head_dim > 0x7fffffffu) {
         return fail(SYN_HIP_EUNSUPPORTED, "attend_tree: max_ctx %u, %u heads", c.max_ctx, d->n_heads);
     }
     if (mask_offset == no_offset) {

@@ -268,9 +268,11 @@ struct attend_rows_args {
     const uint32_t* mask;    // n rows of mask_words words
     uint32_t mask_words;
     uint32_t n, pos, n_kv, group, hd, q_row;
+    uint32_t inv_group;      // 2^32 / group, rounded up
     uint32_t row, ctx_stride;                                // binary16 state
     uint32_t tiles_per_head, tile_bytes, v_at, ks_at, vs_at; // 8-bit state
-    uint32_t wave_tiles, block_rows, row_blocks, chunk, splits;  // attend_plan
+    attend_kernel kernel;                                    // attend_plan
+    uint32_t block_rows, row_blocks, chunk, splits;
     float scale_log2e;
     bool q_f16;
 };

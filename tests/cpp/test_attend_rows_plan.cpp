@@ -42,10 +42,10 @@ int main() {
         const uint32_t n = upto(max_ctx), max_n = n + upto(100) - 1;
         const uint32_t len = n + (max_ctx > n ? static_cast<uint32_t>(r()) % (max_ctx - n + 1) : 0);
         const bool by_pairs = i % 3 == 0;
-        const syn::attend_plan p = syn::plan_attend_rows(n, group, n_kv, len, by_pairs);
-        CHECK(!by_pairs || p.wave_tiles <= 1);
-        CHECK(p.wave_tiles <= 2 && p.block_rows == (p.wave_tiles == 0 ? 16 : 64 * p.wave_tiles));
-        CHECK(p.wave_tiles > 0 || p.row_blocks == 1);
+        const syn::attend_plan p = syn::plan_attend_rows(n, group, n_kv, hd, len, by_pairs);
+        CHECK(!by_pairs || p.kernel <= syn::attend_many16);
+        CHECK(p.kernel != syn::attend_turns || hd <= 128);
+        CHECK(p.kernel != syn::attend_few || p.row_blocks == 1);
         CHECK(uint64_t{p.row_blocks} * p.block_rows >= uint64_t{n} * group);
         CHECK(uint64_t{p.row_blocks - 1} * p.block_rows < uint64_t{n} * group);
         const uint32_t tiles = (len + 63) / 64;
