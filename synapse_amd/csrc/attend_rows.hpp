@@ -185,30 +185,25 @@ __device__ __forceinline__ void store_part(const attend_rows_args& a, const bloc
     *reinterpret_cast<f2*>(a.part_ml + ((size_t{b.split} * a.n_kv + b.g) * (a.n * a.group) + r) * 2) = f2{m, l};
 }
 
-// The order of stream_operands for the scheduler: a pair's products, two
-// reads, and what goes between (vector work and LDS writes).
-template <int AHEAD, int N, int O, class SHAPE>
+// The order of stream_operands for the scheduler: a pair's products, two reads.
+template <int AHEAD, int N, int O, class PRODUCTS>
 __device__ __forceinline__ void sched_pairs() {
     if constexpr (O < N) {
-        __builtin_amdgcn_sched_group_barrier(0x008, SHAPE::products(O), 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS::at(O), 0);
         if constexpr (O + AHEAD < N) {
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
-        if constexpr (SHAPE::valu(O) > 0) {
-            __builtin_amdgcn_sched_group_barrier(0x002, SHAPE::valu(O), 0);
-            __builtin_amdgcn_sched_group_barrier(0x200, 2, 0);
-        }
-        sched_pairs<AHEAD, N, O + 2, SHAPE>();
+        sched_pairs<AHEAD, N, O + 2, PRODUCTS>();
     }
 }
 
-// N operands from LDS, used in pairs: `AHEAD` reads are in flight before the
-// first use, and each pair's use is followed by two more and by between(o).
-// Left to itself the compiler reads a pair, waits for it, and only then reads
-// the next one, which left the matrix units idle for as long as they worked.
-// SHAPE: the products of the pair at o, the vector work of between(o).
-template <int AHEAD, int N, class SHAPE, class READ, class USE, class BETWEEN>
-__device__ __forceinline__ void stream_operands(READ read, USE use, BETWEEN between) {
+// N operands from LDS, used in pairs: AHEAD reads are in flight before the
+// first use, and each pair's use is followed by two more. Left to itself the
+// compiler reads a pair, waits for it, and only then reads the next one, which
+// left the matrix units idle for as long as they worked. PRODUCTS: how many
+// the pair at o has.
+template <int AHEAD, int N, class PRODUCTS, class READ, class USE>
+__device__ __forceinline__ void stream_operands(READ read, USE use) {
     static_assert(AHEAD % 2 == 0 && N % 2 == 0 && AHEAD <= N);
     h8 f[AHEAD];
     __builtin_amdgcn_sched_barrier(0);
@@ -224,10 +219,9 @@ __device__ __forceinline__ void stream_operands(READ read, USE use, BETWEEN betw
             f[o % AHEAD + 1] = read(o + AHEAD + 1);
         }
         use(o, x, y);
-        between(o);
     }
     __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);  // LDS reads
-    sched_pairs<AHEAD, N, 0, SHAPE>();
+    sched_pairs<AHEAD, N, 0, PRODUCTS>();
     __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -447,13 +441,9 @@ struct wave_rows {
     // o % DT of key half o / DT, of K score tile o % 4 of k-step o / 4: what
     // neighbouring products add to lies apart.
     static constexpr int v_ops = 4 * DC, k_ops = 4 * DC;
-    struct v_shape {
-        static constexpr int products(int) { return 4 * RT; }
-        static constexpr int valu(int) { return 0; }
-    };
-    struct k_shape {
-        static constexpr int products(int) { return 2 * RT; }
-        static constexpr int valu(int) { return 0; }
+    template <int FIRST_K>  // operands from FIRST_K on are K's
+    struct products {
+        static constexpr int at(int o) { return o < FIRST_K ? 4 * RT : 2 * RT; }
     };
     __device__ static __forceinline__ h8 read_v(const h8* v_from, int o) {
         return v_from[(o % DT * 2 + o / DT) * 64];
@@ -489,40 +479,23 @@ struct wave_rows {
     }
     template <int AHEAD>
     __device__ __forceinline__ void stream_k(const h8* k_from, f4 (&s)[RT][4], bool k_in) {
-        stream_operands<AHEAD, k_ops, k_shape>([&](int o) { return read_k(k_from, o); },
-                                               [&](int o, h8 x, h8 y) { use_k(o, x, y, s, k_in); }, [](int) {});
+        stream_operands<AHEAD, k_ops, products<0>>([&](int o) { return read_k(k_from, o); },
+                                                   [&](int o, h8 x, h8 y) { use_k(o, x, y, s, k_in); });
     }
     template <int AHEAD>
     __device__ __forceinline__ void stream_v(const h8* v_from) {
-        stream_operands<AHEAD, v_ops, v_shape>([&](int o) { return read_v(v_from, o); },
-                                               [&](int o, h8 x, h8 y) { use_v(o, x, y); }, [](int) {});
+        stream_operands<AHEAD, v_ops, products<v_ops>>([&](int o) { return read_v(v_from, o); },
+                                                       [&](int o, h8 x, h8 y) { use_v(o, x, y); });
     }
-    // Both, with UNITS pieces of other work between: between(i) is two LDS
-    // writes and UNIT_VALU vector instructions.
-    template <int UNITS, int UNIT_VALU>
-    struct vk_shape {
-        static constexpr int unit(int o) {  // of the pair at o, or -1: spread over V's products
-            const int every = v_ops / 2 / (UNITS + 1) * 2;
-            return every > 0 && o % every == 0 && o / every >= 1 && o / every <= UNITS ? o / every - 1 : -1;
-        }
-        static constexpr int products(int o) { return o < v_ops ? 4 * RT : 2 * RT; }
-        static constexpr int valu(int o) { return unit(o) >= 0 ? UNIT_VALU : 0; }
-    };
-    template <int AHEAD, class SHAPE, class BETWEEN>
-    __device__ __forceinline__ void stream_vk(const h8* v_from, const h8* k_from, f4 (&s)[RT][4], bool k_in,
-                                              BETWEEN between) {
-        stream_operands<AHEAD, v_ops + k_ops, SHAPE>(
+    template <int AHEAD>
+    __device__ __forceinline__ void stream_vk(const h8* v_from, const h8* k_from, f4 (&s)[RT][4], bool k_in) {
+        stream_operands<AHEAD, v_ops + k_ops, products<v_ops>>(
             [&](int o) { return o < v_ops ? read_v(v_from, o) : read_k(k_from, o - v_ops); },
             [&](int o, h8 x, h8 y) {
                 if (o < v_ops) {
                     use_v(o, x, y);
                 } else {
                     use_k(o - v_ops, x, y, s, k_in);
-                }
-            },
-            [&](int o) {
-                if (SHAPE::unit(o) >= 0) {
-                    between(SHAPE::unit(o));
                 }
             });
     }
@@ -1054,19 +1027,19 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
 
 // ---- many rows: two groups of waves that take turns -----------------------------
 // Eight waves of 32 rows; waves w and w + 4 share a SIMD. Between two barriers
-// one group is in its matrix products (P V of a tile and K Q of the next),
-// bringing tiles on the side, the other in its exponentials, so that a SIMD's
-// matrix and vector units work at the same time; waves left to themselves
-// were found in the same phase (matrix units 39 % busy, vector units 47 %, and
-// hardly ever both). In interval 2 i group 0 takes the softmax of tile i, in
-// 2 i + 1 its products; group 1 is one interval behind. The products of tile i
-// read V(i) and K(i + 1), in buffers of their parity, in intervals 2 i + 1 and
-// 2 i + 2. With the products of tile i, group 0 brings K(i + 2), in 2 i + 1,
-// and group 1 V(i + 1), in 2 i + 2: each after the last read of what was there
-// (K(i) in 2 i, V(i - 1) in 2 i) and before the first of what comes (2 i + 3).
-// Group 1 also brings an 8-bit tile's steps(i + 2), in 2 i + 2; a group reads
-// steps(i + 1) into registers at the end of its products of tile i, in 2 i + 1
-// and 2 i + 2, those of i being in registers by 2 i.
+// one group is in its matrix products (P V of a tile and K Q of the next), the
+// other in its exponentials and in bringing tiles, so that a SIMD's matrix and
+// vector units work at the same time; waves left to themselves were found in
+// the same phase (matrix units 39 % busy, vector units 47 %, and hardly ever
+// both). In interval 2 i group 0 takes the softmax of tile i, in 2 i + 1 its
+// products; group 1 is one interval behind. The products of tile i read V(i)
+// and K(i + 1), in buffers of their parity, in intervals 2 i + 1 and 2 i + 2.
+// With the softmax of tile i, group 0 brings K(i + 1), in 2 i, and group 1
+// V(i + 1), in 2 i + 1: each after the last read of what was there (K(i - 1)
+// in 2 i - 2, V(i - 1) in 2 i) and before the first of what comes (2 i + 1, 2 i
+// + 3). An 8-bit tile's steps(i + 2) come with group 1's products of tile i, in
+// 2 i + 2; a group reads steps(i + 1) into registers at the end of its products
+// of tile i, in 2 i + 1 and 2 i + 2, those of i being in registers by 2 i.
 template <int DC, bool EIGHT, bool TREE>
 __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_args a) {
     using namespace attend;
@@ -1079,8 +1052,7 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
 
     const uint32_t lane = threadIdx.x % 64, in_group = threadIdx.x % 256;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const bool k_group = w < 4;               // group 0: brings K
-    const uint32_t ahead = k_group ? 2 : 1;   // tiles ahead of its products
+    const bool k_group = w < 4;  // group 0: brings K
     const block_place b = place_block<TREE>(a);
     const uint32_t n_rows = a.n * a.group;
     const uint32_t row0 = b.row0 + w * (RT * 16);
@@ -1098,8 +1070,7 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
     int run_vexp = no_vexp;  // wave 4's: the steps' power of two up to the staged tile
 
     // This group's part (K or V) of a tile: 8-bit loads into registers, to be
-    // staged; binary16 copies straight to their buffer. Wave 4 loads the steps
-    // one tile further on.
+    // staged; binary16 copies straight to their buffer.
     const auto load = [&](uint32_t tile) {
         if constexpr (EIGHT) {
             const uint8_t* t = head + size_t{tile} * a.tile_bytes + (k_group ? 0 : a.v_at);
@@ -1125,22 +1096,30 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
             }
         }
     };
-    const auto stage_unit = [&](uint32_t tile, int i) {
-        h8* to = k_group ? &k_lds[tile & 1][0][0] : &v_lds[tile & 1][0][0];
-        const uint32_t u = i * 256 + in_group;
-        uint32_t at = u / 64 * 128 + u % 64, then = 64;  // V, and K of whole 64s of dims
-        if (DC % 2 != 0 && k_group) {
-            const uint32_t st = u / (32 * DC), rest = u % (32 * DC);
-            if (rest < 64 * KQ) {
-                at = (st * DC + rest / 64 * 2) * 64 + rest % 64;
-            } else {  // an odd last 32: 8 dims of two keys
-                at = (st * DC + DC - 1) * 64 + (rest - 64 * KQ) * 2;
-                then = 1;
+    // What load started, to its buffer (and waited for).
+    const auto stage = [&](uint32_t tile) {
+        if constexpr (EIGHT) {
+            h8* to = k_group ? &k_lds[tile & 1][0][0] : &v_lds[tile & 1][0][0];
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const uint32_t u = i * 256 + in_group;
+                uint32_t at = u / 64 * 128 + u % 64, then = 64;  // V, and K of whole 64s of dims
+                if (DC % 2 != 0 && k_group) {
+                    const uint32_t st = u / (32 * DC), rest = u % (32 * DC);
+                    if (rest < 64 * KQ) {
+                        at = (st * DC + rest / 64 * 2) * 64 + rest % 64;
+                    } else {  // an odd last 32: 8 dims of two keys
+                        at = (st * DC + DC - 1) * 64 + (rest - 64 * KQ) * 2;
+                        then = 1;
+                    }
+                }
+                if (DC % 2 == 0 || u < 128 * DC) {
+                    to[at] = bytes_h8(next[i][0], next[i][1]);
+                    to[at + then] = bytes_h8(next[i][2], next[i][3]);
+                }
             }
-        }
-        if (DC % 2 == 0 || u < 128 * DC) {
-            to[at] = bytes_h8(next[i][0], next[i][1]);
-            to[at + then] = bytes_h8(next[i][2], next[i][3]);
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
     };
     const auto load_steps = [&](uint32_t tile) {
@@ -1187,38 +1166,20 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
     const bool k_in = (DC - 1) * 32 + lane / 16 * 8 < a.hd;
     const uint32_t t0 = b.t_begin, t1 = b.t_end;
     if (t0 < t1) {  // (a split of a causal run may lie behind all keys of these rows)
-        // Before the turns: K of the first two tiles, V of the first, steps of
-        // both; the first scores; the loads that the first products stage.
+        // Before the turns: the first tile, its steps and the second one's; the
+        // first scores; the loads that the first softmax stages.
         typename wave_rows_t::raw_q raw;
         rows.load_q(a, b, raw);
         load(t0);
         load_steps(t0);
-        if constexpr (EIGHT) {
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                stage_unit(t0, i);
-            }
-            stage_steps(t0);
-            load_steps(t0 + 1);
-        }
-        if (k_group && t0 + 1 < t1) {
+        stage(t0);
+        stage_steps(t0);
+        load_steps(t0 + 1);
+        stage_steps(t0 + 1);
+        if (EIGHT && t0 + 1 < t1) {
             load(t0 + 1);
-            if constexpr (EIGHT) {
-#pragma unroll
-                for (int i = 0; i < LOADS; ++i) {
-                    stage_unit(t0 + 1, i);
-                }
-            }
         }
-        if constexpr (EIGHT) {
-            stage_steps(t0 + 1);
-            if (t0 + ahead < t1) {
-                load(t0 + ahead);
-            }
-            load_steps(t0 + 2);
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
+        load_steps(t0 + 2);
         rows.take_q(a, b, raw);
         turn();
         read_steps(t0);
@@ -1233,6 +1194,10 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
             constexpr bool MASKED = decltype(masked)::value;
             for (uint32_t tile = from; tile < to; ++tile) {
                 const uint32_t key0 = tile * attend_tile;
+                const bool more = tile + 1 < t1;
+                if (!EIGHT && more) {
+                    load(tile + 1);
+                }
                 if (key0 < reach) {
                     if constexpr (EIGHT) {
                         rows.raise_vexp(__builtin_amdgcn_readfirstlane(vexp));
@@ -1243,46 +1208,28 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
                                                       [](int) { return 1.0f; });
                     }
                 }
+                if (more) {
+                    stage(tile + 1);
+                }
+                if (EIGHT && tile + 2 < t1) {
+                    load(tile + 2);
+                }
                 turn();
                 __builtin_amdgcn_s_setprio(1);
-                const uint32_t bring = tile + ahead;
-                if (!EIGHT && bring < t1) {
-                    load(bring);
-                }
-                // (The last tiles stage what is not read, and behind the last
-                // one the scores are not used: one path for every tile.)
-                const h8* v_from = &v_lds[tile & 1][0][lane];
-                const h8* k_from = &k_lds[(tile + 1) & 1][0][lane];
-                if constexpr (!EIGHT && MASKED) {
-                    if (key0 < reach) {
+                if (key0 < reach) {  // (behind the last tile the scores are not used)
+                    const h8* v_from = &v_lds[tile & 1][0][lane];
+                    const h8* k_from = &k_lds[(tile + 1) & 1][0][lane];
+                    if constexpr (!EIGHT && MASKED) {
                         rows.add_tail(v_from, key0, b.len);
                         rows.template stream_k<4>(k_from, s, k_in);
-                    }
-                } else if (key0 < reach) {
-                    typedef typename wave_rows_t::template vk_shape<EIGHT && DC % 2 == 0 ? LOADS : 0, 16> shape;
-                    rows.template stream_vk<6, shape>(v_from, k_from, s, k_in,
-                                                      [&](int i) { stage_unit(bring, i); });
-                    if constexpr (EIGHT && DC % 2 != 0) {
-#pragma unroll
-                        for (int i = 0; i < LOADS; ++i) {
-                            stage_unit(bring, i);
-                        }
-                    }
-                } else if constexpr (EIGHT) {
-#pragma unroll
-                    for (int i = 0; i < LOADS; ++i) {
-                        stage_unit(bring, i);
+                    } else {
+                        rows.template stream_vk<6>(v_from, k_from, s, k_in);
                     }
                 }
                 if constexpr (EIGHT) {
                     stage_steps(tile + 2);
-                    if (bring + 1 < t1) {
-                        load(bring + 1);
-                    }
                     load_steps(tile + 3);
                     read_steps(tile + 1);
-                } else {
-                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 }
                 __builtin_amdgcn_s_setprio(0);
                 turn();
