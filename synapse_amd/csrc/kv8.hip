@@ -23,16 +23,6 @@ namespace {
 constexpr uint32_t threads = 512;
 constexpr uint32_t max_record = kv8_tile * 256;  // K or V bytes of a tile at hd 256
 
-// The key whose value is in byte b of a tile's K block, and likewise V.
-__device__ __forceinline__ uint32_t k_key(uint32_t b, uint32_t hdp) {
-    const uint32_t op = b / (16 * hdp), rest = b % (16 * hdp), pairs = hdp / 64 * 64;
-    const uint32_t m = rest < pairs * 16 ? rest / 16 % 16 : (rest - pairs * 16) / 8 % 16;
-    return op / 2 * 32 + m / 4 * 8 + op % 2 * 4 + m % 4;
-}
-__device__ __forceinline__ uint32_t v_key(uint32_t b) {
-    return b % 16 / 8 * 32 + b % 1024 / 256 * 8 + b % 8;
-}
-
 // Four values of a row, from dim d0 on (zeros past the last one).
 template <typename T>
 __device__ __forceinline__ f4 load_four(const T* row, uint32_t d0, uint32_t hd, bool vec) {
@@ -95,101 +85,151 @@ __device__ __forceinline__ uint32_t group_max(uint32_t u) {
     return u;
 }
 
-// x / d to the nearest whole number, ties to even, for |x| up to 127.5 d.
-__device__ __forceinline__ int quotient(float x, float d) {
+// A row's four values of this lane over its step: whole numbers + 128, a byte
+// each. inv is next to 1 / d, so x inv is off by some 2^-22: rounded, it is the
+// quotient's nearest whole number or, next to a half, that number's neighbour.
+// The remainder tells which, exactly (a multiple of half an ulp of d, not over
+// d, so the fused multiply-add does not round it); only where some lane's
+// reaches half a step is there anything to put right.
+__device__ __forceinline__ uint32_t quotients(f4 x, float step) {
 #pragma clang fp contract(off)
-    float q = rintf(x / d);
-    const float r = __builtin_fmaf(-q, d, x);  // exact: a multiple of half an ulp of d, not over d
-    const float twice = 2.0f * fabsf(r);
-    const bool odd = (static_cast<int>(q) & 1) != 0;
-    if (twice > d || (twice == d && odd)) {
-        q += copysignf(1.0f, r);
+    float d = step;
+    const bool small = step < 0x1p-100f;  // its inverse may be out of range: row and step times 2^64, exactly
+    if (__builtin_amdgcn_ballot_w64(small && step != 0.0f) != 0) {
+        const float up = small ? 0x1p64f : 1.0f;
+        d *= up;
+        x *= up;
     }
-    return static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f));
+    const float inv = __builtin_amdgcn_rcpf(d), half = 0.5f * d;
+    float q[4], r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        q[e] = rintf(x[e] * inv);
+        r[e] = __builtin_fmaf(-q[e], d, x[e]);
+    }
+    const float most = fmaxf(fmaxf(fabsf(r[0]), fabsf(r[1])), fmaxf(fabsf(r[2]), fabsf(r[3])));
+    if (__builtin_amdgcn_ballot_w64(most >= half) != 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool odd = (static_cast<int>(q[e]) & 1) != 0;
+            const float ar = fabsf(r[e]);
+            q[e] += ar > half || (ar == half && odd) ? copysignf(1.0f, r[e]) : 0.0f;
+        }
+    }
+    uint32_t bytes = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        bytes = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_amdgcn_fmed3f(q[e], -127.0f, 127.0f) + 128.0f, e, bytes);
+    }
+    return bytes;
 }
 
 // grid: tiles of the run x KV heads, KV heads fastest; block 512. LANES: hd /
-// 4 rounded up to a power of two.
+// 4 rounded up to a power of two. A group of LANES lanes takes K or V of four
+// neighbouring keys at a time, so that a lane has a word of each key's K and
+// of each dim's V. Tiles that are the run's whole go through LDS as whole
+// lines; of the first and last, K's words are written straight to the record,
+// and V's through LDS, by words where all four keys are the run's. Up to four
+// keys (a decode step) write V's bytes straight too: no barrier.
 template <typename T, int LANES>
 __global__ __launch_bounds__(threads) void kv8_append_kernel(const kv8_rows_args a, uint32_t tile0, bool vec) {
     __shared__ __align__(16) uint8_t lds[2][max_record];
-    __shared__ float steps[2][kv8_tile];
     const kv8_shape& s = a.shape;
     const uint32_t g = blockIdx.x % s.n_kv, tile = tile0 + blockIdx.x / s.n_kv;
     const uint32_t key0 = tile * kv8_tile, end = a.pos0 + a.n;
     const uint32_t from = key0 < a.pos0 ? a.pos0 - key0 : 0;             // the tile's keys that the run writes
     const uint32_t to = end - key0 < kv8_tile ? end - key0 : kv8_tile;
+    const bool whole = from == 0 && to == kv8_tile, few = to - from <= 4;
     const uint32_t in_group = threadIdx.x % LANES, d0 = in_group * 4;
+    constexpr uint32_t per_wave = 64 / LANES, groups = threads / LANES / 2;  // for K, and as many for V
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t which = w % 2;                                            // 0 K, 1 V
+    const uint32_t group = w / 2 * per_wave + threadIdx.x % 64 / LANES;
     const size_t row = size_t{s.n_kv} * s.hd;
-    constexpr uint32_t groups = threads / LANES;
+    const T* in = static_cast<const T*>(which ? a.v_in : a.k_in) + size_t{g} * s.hd;
+    uint8_t* rec = a.kv8 + (size_t{g} * s.tiles + tile) * s.tile_bytes;
+    float* steps = reinterpret_cast<float*>(rec + (which ? s.vs_at : s.ks_at));
 
-    // Rows 2 key + (0 K, 1 V); each group takes every groups-th.
-    for (uint32_t i = 2 * from + threadIdx.x / LANES; i < 2 * to; i += groups) {
-        const uint32_t key = i / 2, which = i % 2;
-        const T* src = static_cast<const T*>(which ? a.v_in : a.k_in) + (key0 + key - a.pos0) * row + size_t{g} * s.hd;
-        const f4 x = load_four(src, d0, s.hd, vec);
-        uint32_t top = 0;  // of the magnitudes' bits, which are in their order, NaN above all
+#pragma unroll 1
+    for (uint32_t key4 = from / 4 * 4 + group * 4; key4 < to; key4 += groups * 4) {
+        f4 x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float xe = x[e];  // (a bit cast of the element itself casts element 0)
-            const uint32_t b = __builtin_bit_cast(uint32_t, xe) & 0x7fffffffu;
-            top = b > top ? b : top;
-        }
-        top = group_max<LANES>(top);
-        const bool wild = top >= 0x7f800000u;
-        const float d = __builtin_bit_cast(float, top) / 127.0f;
-        uint32_t bytes = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int q = wild || d == 0.0f ? 0 : quotient(x[e], d);
-            bytes |= static_cast<uint32_t>(q + 128) << (8 * e);
-        }
-        if (d0 < s.hdp) {
-            if (which == 0) {
-                *reinterpret_cast<uint32_t*>(&lds[0][kv8_k_at(s.hdp, key, d0)]) = bytes;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    lds[1][kv8_v_at(key, d0 + e)] = static_cast<uint8_t>(bytes >> (8 * e));
-                }
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (key4 + i >= from && key4 + i < to) {
+                x[i] = load_four(in + (key0 + key4 + i - a.pos0) * row, d0, s.hd, vec);
             }
         }
-        if (in_group == 0) {
-            steps[which][key] = wild ? __builtin_nanf("") : d;
-        }
-    }
-    __syncthreads();
-
-    uint8_t* rec = a.kv8 + (size_t{g} * s.tiles + tile) * s.tile_bytes;
-    const uint32_t bytes = kv8_tile * s.hdp;
-    if (from == 0 && to == kv8_tile) {
-        for (uint32_t i = threadIdx.x * 16; i < 2 * bytes; i += threads * 16) {
-            const uint32_t which = i >= bytes, b = i - which * bytes;
-            store16(rec + i, *reinterpret_cast<const u4*>(&lds[which][b]));
-        }
-    } else {
-        // Only the run's keys: a word of K is one key's, a word of V four
-        // keys', stored by the byte where some of them are not the run's.
-        for (uint32_t i = threadIdx.x * 4; i < 2 * bytes; i += threads * 4) {
-            const uint32_t which = i >= bytes, b = i - which * bytes;
-            const uint32_t key = which ? v_key(b) : k_key(b, s.hdp);
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(&lds[which][b]);
-            if (key >= from && key + (which ? 3 : 0) < to) {
-                *reinterpret_cast<uint32_t*>(rec + i) = x;
-            } else if (which) {
+        uint32_t bytes[4];
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) {
-                    if (key + e >= from && key + e < to) {
-                        rec[i + e] = static_cast<uint8_t>(x >> (8 * e));
+        for (uint32_t i = 0; i < 4; ++i) {
+            uint32_t top = 0;  // of the magnitudes' bits, which are in their order, NaN above all
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float xe = x[i][e];  // (a bit cast of the element itself casts element 0)
+                const uint32_t b = __builtin_bit_cast(uint32_t, xe) & 0x7fffffffu;
+                top = b > top ? b : top;
+            }
+            top = group_max<LANES>(top);
+            const bool wild = top >= 0x7f800000u;
+            const float step = __builtin_bit_cast(float, top) / 127.0f;
+            const uint32_t q = quotients(x[i], step);
+            bytes[i] = wild || step == 0.0f ? 0x80808080u : q;
+            if (in_group == 0 && key4 + i >= from && key4 + i < to) {
+                steps[key4 + i] = wild ? __builtin_nanf("") : step;
+            }
+        }
+        if (d0 >= s.hdp) {
+            continue;
+        }
+        if (which == 0) {
+            uint8_t* k = whole ? lds[0] : rec;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                if (key4 + i >= from && key4 + i < to) {
+                    *reinterpret_cast<uint32_t*>(k + kv8_k_at(s.hdp, key4 + i, d0)) = bytes[i];
+                }
+            }
+        } else if (!few) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t v = (bytes[0] >> (8 * e) & 0xff) | (bytes[1] >> (8 * e) & 0xff) << 8 |
+                                   (bytes[2] >> (8 * e) & 0xff) << 16 | (bytes[3] >> (8 * e) & 0xff) << 24;
+                *reinterpret_cast<uint32_t*>(lds[1] + kv8_v_at(key4, d0 + e)) = v;
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                if (key4 + i >= from && key4 + i < to) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        rec[s.v_at + kv8_v_at(key4 + i, d0 + e)] = static_cast<uint8_t>(bytes[i] >> (8 * e));
                     }
                 }
             }
         }
     }
-    if (threadIdx.x < 2 * kv8_tile) {
-        const uint32_t which = threadIdx.x / kv8_tile, key = threadIdx.x % kv8_tile;
-        if (key >= from && key < to) {
-            *reinterpret_cast<float*>(rec + (which ? s.vs_at : s.ks_at) + key * 4) = steps[which][key];
+    if (whole) {
+        __syncthreads();
+        const uint32_t bytes = kv8_tile * s.hdp;
+        for (uint32_t i = threadIdx.x * 16; i < 2 * bytes; i += threads * 16) {
+            const uint32_t in_v = i >= bytes, b = i - in_v * bytes;
+            store16(rec + i, *reinterpret_cast<const u4*>(&lds[in_v][b]));
+        }
+    } else if (!few) {
+        __syncthreads();
+        for (uint32_t b = threadIdx.x * 4; b < kv8_tile * s.hdp; b += threads * 4) {
+            const uint32_t key = b % 16 / 8 * 32 + b % 1024 / 256 * 8 + b % 8;  // (kv8_v_at the other way)
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(&lds[1][b]);
+            if (key >= from && key + 3 < to) {
+                *reinterpret_cast<uint32_t*>(rec + s.v_at + b) = x;
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    if (key + e >= from && key + e < to) {
+                        rec[s.v_at + b + e] = static_cast<uint8_t>(x >> (8 * e));
+                    }
+                }
+            }
         }
     }
 }
@@ -206,38 +246,58 @@ __global__ __launch_bounds__(threads) void kv8_read_kernel(const kv8_rows_args a
     const uint32_t to = end - key0 < kv8_tile ? end - key0 : kv8_tile;
     const uint8_t* rec = a.kv8 + (size_t{g} * s.tiles + tile) * s.tile_bytes;
     const uint32_t bytes = kv8_tile * s.hdp;
-    for (uint32_t i = threadIdx.x * 16; i < 2 * bytes; i += threads * 16) {
-        const uint32_t which = i >= bytes;
-        *reinterpret_cast<u4*>(&lds[which][i - which * bytes]) = load16(rec + i);
+    constexpr uint32_t most = 2 * kv8_tile * 4 * LANES / (threads * 16);
+    u4 x[most];
+#pragma unroll
+    for (uint32_t i = 0; i < most; ++i) {
+        const uint32_t at = (i * threads + threadIdx.x) * 16;
+        if (at < 2 * bytes) {
+            x[i] = load16(rec + at);
+        }
     }
     if (threadIdx.x < 2 * kv8_tile) {
         const uint32_t which = threadIdx.x / kv8_tile, key = threadIdx.x % kv8_tile;
         steps[which][key] = *reinterpret_cast<const float*>(rec + (which ? s.vs_at : s.ks_at) + key * 4);
     }
+#pragma unroll
+    for (uint32_t i = 0; i < most; ++i) {
+        const uint32_t at = (i * threads + threadIdx.x) * 16;
+        if (at < 2 * bytes) {
+            const uint32_t which = at >= bytes;
+            *reinterpret_cast<u4*>(&lds[which][at - which * bytes]) = x[i];
+        }
+    }
     __syncthreads();
     const uint32_t d0 = threadIdx.x % LANES * 4;
-    const size_t row = size_t{s.n_kv} * s.hd;
     if (d0 >= s.hd) {
         return;
     }
-    constexpr uint32_t groups = threads / LANES;
-    for (uint32_t i = 2 * from + threadIdx.x / LANES; i < 2 * to; i += groups) {
-        const uint32_t key = i / 2, which = i % 2;
-        uint32_t b;
-        if (which == 0) {
-            b = *reinterpret_cast<const uint32_t*>(&lds[0][kv8_k_at(s.hdp, key, d0)]);
-        } else {
-            b = lds[1][kv8_v_at(key, d0)] | lds[1][kv8_v_at(key, d0 + 1)] << 8 |
-                lds[1][kv8_v_at(key, d0 + 2)] << 16 | static_cast<uint32_t>(lds[1][kv8_v_at(key, d0 + 3)]) << 24;
-        }
-        const float d = steps[which][key];
-        f4 x;
+    constexpr uint32_t per_wave = 64 / LANES, groups = threads / LANES / 2;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t which = w % 2;
+    const uint32_t group = w / 2 * per_wave + threadIdx.x % 64 / LANES;
+    const size_t row = size_t{s.n_kv} * s.hd;
+    T* out = static_cast<T*>(which ? a.v_out : a.k_out) + size_t{g} * s.hd;
+    for (uint32_t key4 = from / 4 * 4 + group * 4; key4 < to; key4 += groups * 4) {
+        uint32_t b[4];  // K: of key i, V: of dim i
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[e] = static_cast<float>(static_cast<int>(b >> (8 * e) & 0xff) - 128) * d;
+        for (uint32_t i = 0; i < 4; ++i) {
+            b[i] = *reinterpret_cast<const uint32_t*>(which ? &lds[1][kv8_v_at(key4, d0 + i)]
+                                                            : &lds[0][kv8_k_at(s.hdp, key4 + i, d0)]);
         }
-        store_four(static_cast<T*>(which ? a.v_out : a.k_out) + (key0 + key - a.pos0) * row + size_t{g} * s.hd, d0,
-                   s.hd, vec, x);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (key4 + i >= from && key4 + i < to) {
+                const float d = steps[which][key4 + i];
+                f4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t q = which ? b[e] >> (8 * i) & 0xff : b[i] >> (8 * e) & 0xff;
+                    x[e] = static_cast<float>(static_cast<int>(q) - 128) * d;
+                }
+                store_four(out + (key0 + key4 + i - a.pos0) * row, d0, s.hd, vec, x);
+            }
+        }
     }
 }
 
