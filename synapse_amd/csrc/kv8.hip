@@ -353,9 +353,16 @@ struct read_rows {
 // handful of rows of a few KB: bound by two dependent trips to memory.
 constexpr uint32_t batch = 8;
 
-template <typename T, class AT>
-__device__ __forceinline__ void move_column(AT at, uint32_t first, uint32_t count, const keep_rows& r) {
-    for (uint32_t i0 = 0; i0 < count; i0 += batch) {
+// A launch of up to `batch` rows (an accepted path) carries them in an argument
+// block of 16 bytes, read with the other arguments.
+struct few_rows {
+    uint16_t row[batch];
+};
+
+template <typename T, class ROWS, class AT>
+__device__ __forceinline__ void move_column(AT at, uint32_t first, uint32_t count, const ROWS& r) {
+    constexpr uint32_t most = sizeof(r.row) / sizeof(r.row[0]);
+    for (uint32_t i0 = 0; i0 < (most == batch ? 1 : count); i0 += batch) {
         T x[batch];
 #pragma unroll
         for (uint32_t i = 0; i < batch; ++i) {
@@ -372,8 +379,9 @@ __device__ __forceinline__ void move_column(AT at, uint32_t first, uint32_t coun
     }
 }
 
+template <class ROWS>
 __global__ __launch_bounds__(256) void kv_keep_kernel(const kv_layout c, uint32_t pos, uint32_t first, uint32_t count,
-                                                      const keep_rows r) {
+                                                      const ROWS r) {
     const uint32_t row = c.n_kv * c.hd;  // even, as hd is
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;
     if (i < row / 2) {
@@ -385,15 +393,15 @@ __global__ __launch_bounds__(256) void kv_keep_kernel(const kv_layout c, uint32_
     }
 }
 
+template <class ROWS>
 __global__ __launch_bounds__(256) void kv8_keep_kernel(uint8_t* kv8, const kv8_shape s, uint32_t pos, uint32_t first,
-                                                       uint32_t count, const keep_rows r) {
+                                                       uint32_t count, const ROWS r) {
     const uint32_t words = s.hdp / 4, columns = words + s.hd + 2;  // a KV head's: K words, V bytes, steps
-    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-    const uint32_t g = i / columns, j = i % columns;
-    if (g >= s.n_kv) {
+    const uint32_t j = blockIdx.y * 256 + threadIdx.x;
+    if (j >= columns) {
         return;
     }
-    uint8_t* head = kv8 + size_t{g} * s.tiles * s.tile_bytes;
+    uint8_t* head = kv8 + size_t{blockIdx.x} * s.tiles * s.tile_bytes;
     const auto rec = [=](uint32_t t) { return head + size_t{(pos + t) / kv8_tile} * s.tile_bytes; };
     if (j < words) {
         move_column<uint32_t>(
@@ -412,6 +420,14 @@ __global__ __launch_bounds__(256) void kv8_keep_kernel(uint8_t* kv8, const kv8_s
     }
 }
 
+few_rows few_of(const keep_rows& rows) {
+    few_rows f{};
+    for (uint32_t i = 0; i < batch; ++i) {
+        f.row[i] = rows.row[i];
+    }
+    return f;
+}
+
 }  // namespace
 
 hipError_t launch_kv8_append(const kv8_rows_args& a, hipStream_t stream) {
@@ -425,14 +441,23 @@ hipError_t launch_kv8_read(const kv8_rows_args& a, hipStream_t stream) {
 hipError_t launch_kv_keep(const kv_layout& c, uint32_t pos, uint32_t first, uint32_t count, const keep_rows& rows,
                           hipStream_t stream) {
     const uint64_t columns = uint64_t{c.n_kv} * c.hd / 2 * 3;
-    kv_keep_kernel<<<static_cast<uint32_t>((columns + 255) / 256), 256, 0, stream>>>(c, pos, first, count, rows);
+    const uint32_t blocks = static_cast<uint32_t>((columns + 255) / 256);
+    if (count <= batch) {
+        kv_keep_kernel<<<blocks, 256, 0, stream>>>(c, pos, first, count, few_of(rows));
+    } else {
+        kv_keep_kernel<<<blocks, 256, 0, stream>>>(c, pos, first, count, rows);
+    }
     return hipGetLastError();
 }
 
 hipError_t launch_kv8_keep(uint8_t* kv8, const kv8_shape& s, uint32_t pos, uint32_t first, uint32_t count,
                            const keep_rows& rows, hipStream_t stream) {
-    const uint64_t columns = uint64_t{s.n_kv} * (s.hdp / 4 + s.hd + 2);
-    kv8_keep_kernel<<<static_cast<uint32_t>((columns + 255) / 256), 256, 0, stream>>>(kv8, s, pos, first, count, rows);
+    const dim3 blocks(s.n_kv, (s.hdp / 4 + s.hd + 2 + 255) / 256);
+    if (count <= batch) {
+        kv8_keep_kernel<<<blocks, 256, 0, stream>>>(kv8, s, pos, first, count, few_of(rows));
+    } else {
+        kv8_keep_kernel<<<blocks, 256, 0, stream>>>(kv8, s, pos, first, count, rows);
+    }
     return hipGetLastError();
 }
 
