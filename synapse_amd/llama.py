@@ -31,7 +31,7 @@ import numpy as np
 
 from . import capi
 from .capi import (NO_OFFSET, SYN_ADD, SYN_F32, SYN_SILU_MUL, Arena, AttnDesc, AttnRopeDesc, ElementwiseDesc, EmbedDesc,
-                   MatmulDesc, MatmulQDesc, NormDesc, check, lib)
+                   Kv8AttnDesc, MatmulDesc, MatmulQDesc, NormDesc, RopeDesc, TemperatureDesc, check, lib)
 from .gguf import F32, Q4_0, Q4_K, Q5_0, Q6_K, Q8_0, TYPE_NAMES, GGUFError, GGUFFile
 
 _f32 = np.float32
@@ -199,11 +199,14 @@ def _f32_weight(f: GGUFFile, name: str, shape) -> np.ndarray:
 class DeviceLlama:
     """The decode graph on the GPU: one arena holding the weights, the
     activations, the RoPE factors, one KV state per layer and the attention
-    scratch. step(token, pos) runs one token and returns its logits."""
+    scratch. step(token, pos) runs one token and returns its logits. With kv8
+    the KV states are 8-bit ones (syn_kv8_desc), about half the size."""
 
-    def __init__(self, f: GGUFFile, max_ctx: int):
+    kv8 = False
+
+    def __init__(self, f: GGUFFile, max_ctx: int, kv8: bool = False):
         c = self.config = read_config(f)
-        self.max_ctx = max_ctx
+        self.max_ctx, self.kv8 = max_ctx, kv8
         hd, E, F, V = c.head_dim, c.n_embd, c.n_ff, c.n_vocab
         q_rows, kv_rows = c.n_head * hd, c.n_head_kv * hd
         # Tensors that change the result and that this architecture does not
@@ -253,18 +256,21 @@ class DeviceLlama:
         # ---- arena layout: weights, activations, KV states, scratch ----------
         act = {"x": E, "h": E, "q": q_rows, "qr": q_rows, "k": kv_rows, "kr": kv_rows, "v": kv_rows,
                "attn": q_rows, "o": E, "gate": F, "up": F, "down": E, "logits": V}
-        scratch_bytes = int(lib().syn_hip_attention_scratch_bytes(c.n_head, c.n_head_kv, hd, max_ctx, 1))
+        scratch_fn = lib().syn_hip_kv8_attention_scratch_bytes if kv8 else lib().syn_hip_attention_scratch_bytes
+        scratch_bytes = int(scratch_fn(c.n_head, c.n_head_kv, hd, max_ctx, 1))
+        state_bytes = (capi.kv8_state_bytes if kv8 else capi.kv_state_bytes)(max_ctx, c.n_head_kv, hd)
         # One activation-quantization buffer serves every quantized matrix.
         qact_bytes = max([int(lib().syn_hip_matmul_q_act_bytes(t, 1, cols))
                           for t, cols in self.wtype.values() if t != F32] or [0])
         total = sum(capi.align(a.nbytes) for a in self._host.values())
         total += sum(capi.align(n * 4) for n in act.values()) + capi.align(max(qact_bytes, 1))
-        total += c.n_layer * capi.align(capi.kv_state_bytes(max_ctx, c.n_head_kv, hd)) + capi.align(scratch_bytes)
+        total += c.n_layer * capi.align(state_bytes) + capi.align(scratch_bytes)
         self.arena = Arena(total + 4096)
         self.off = {name: self.arena.put(a) for name, a in self._host.items()}
         self.act = {name: self.arena.alloc(n * 4) for name, n in act.items()}
         self.qact = self.arena.alloc(max(qact_bytes, 1))
-        self.caches = [capi.kv_state(self.arena, max_ctx, c.n_head_kv, hd) for _ in range(c.n_layer)]
+        state = capi.kv8_state if kv8 else capi.kv_state
+        self.caches = [state(self.arena, max_ctx, c.n_head_kv, hd) for _ in range(c.n_layer)]
         self.scratch = (self.arena.alloc(scratch_bytes), scratch_bytes)
         self.theta_scale = rope_theta_scale(c.rope_base, hd)
         self.scale = float(_f32(1) / np.sqrt(_f32(hd)))
@@ -276,9 +282,10 @@ class DeviceLlama:
 
     def reset(self) -> None:
         """Zeroes the KV states, as before a new sequence."""
+        state_bytes = capi.kv8_state_bytes if self.kv8 else capi.kv_state_bytes
         for cache in self.caches:
-            self.arena.fill(cache.k_offset, 0, capi.kv_state_bytes(self.max_ctx, self.config.n_head_kv,
-                                                                    self.config.head_dim))
+            self.arena.fill(cache.offset if self.kv8 else cache.k_offset, 0,
+                            state_bytes(self.max_ctx, self.config.n_head_kv, self.config.head_dim))
 
     # ---- one op each, through the C ABI ---------------------------------------
     # The graph's calls and their descriptors are laid out once, with the
@@ -332,12 +339,37 @@ class DeviceLlama:
         self._attn.append(ad)
         self._call("syn_hip_attention_rope", ad, rd)
 
+    def _attention8(self, layer):
+        """The same on an 8-bit state: op_rope on q and on k, op_attn_temperature
+        and syn_hip_kv8_attention, a call each."""
+        c, s = self.config, self.config.rope_scaling
+        for x, out, heads in (("q", "qr", c.n_head), ("k", "kr", c.n_head_kv)):
+            d = RopeDesc(in_offset=self.act[x], out_offset=self.act[out],
+                         freq_factors_offset=self.off[self.freq_factors] if self.freq_factors else NO_OFFSET, n=1,
+                         size=heads * c.head_dim, head_dim=c.head_dim, pos=0, theta_scale=self.theta_scale,
+                         mode=c.rope_mode, freq_scale=s.freq_scale, ext_factor=s.ext_factor, attn_factor=s.attn_factor,
+                         corr_low=s.corr_low, corr_high=s.corr_high)
+            self._at_pos.append(d)
+            self._call("syn_hip_rope", d)
+        if c.attn_temp_scale != 0.0:
+            d = TemperatureDesc(in_offset=self.act["qr"], out_offset=self.act["qr"], n=1, size=c.n_head * c.head_dim,
+                                pos=0, floor_len=c.n_ctx_orig, scale=c.attn_temp_scale)
+            self._at_pos.append(d)
+            self._call("syn_hip_attn_temperature", d)
+        ad = Kv8AttnDesc(cache=self.caches[layer], q_offset=self.act["qr"], k_offset=self.act["kr"],
+                         v_offset=self.act["v"], out_offset=self.act["attn"], scratch_offset=self.scratch[0],
+                         scratch_bytes=self.scratch[1], mask_offset=NO_OFFSET, n_heads=c.n_head, pos=0, n=1,
+                         scale=self.scale, q_dtype=SYN_F32, kv_dtype=SYN_F32)
+        self._attn.append(ad)
+        self._call("syn_hip_kv8_attention", ad)
+
     def _lay_out_graph(self) -> None:
         c = self.config
         hd, E, F, V = c.head_dim, c.n_embd, c.n_ff, c.n_vocab
         q_rows, kv_rows = c.n_head * hd, c.n_head_kv * hd
         self._graph = []  # (entry point, descriptors) of a step behind its embedding
         self._attn = []   # the attention descriptors among them, one per layer
+        self._at_pos = []  # others that take the position
         self._embed = EmbedDesc(table_offset=self.off["token_embd.weight"], out_offset=self.act["x"], n_table_rows=V,
                                 size=E, table_type=self.wtype["token_embd.weight"][0])
         for l in range(c.n_layer):
@@ -346,7 +378,8 @@ class DeviceLlama:
             self._matmul(b + "attn_q.weight", "h", "q", q_rows, E, b + "attn_q.bias")
             self._matmul(b + "attn_k.weight", "h", "k", kv_rows, E, b + "attn_k.bias")
             self._matmul(b + "attn_v.weight", "h", "v", kv_rows, E, b + "attn_v.bias")
-            self._attention(l)  # RoPE, then the temperature after it (llm_build_mistral3), then attention
+            # RoPE, then the temperature after it (llm_build_mistral3), then attention
+            (self._attention8 if self.kv8 else self._attention)(l)
             self._matmul(b + "attn_output.weight", "attn", "o", E, q_rows, b + "attn_output.bias")
             self._elementwise(SYN_ADD, "o", "x", "x", E)
             self._norm("x", b + "ffn_norm.weight", "h")
@@ -368,6 +401,8 @@ class DeviceLlama:
         for ad, cache in zip(self._attn, self.caches, strict=True):
             ad.cache = cache  # (a program may give the model another sequence's states)
             ad.pos = pos
+        for d in self._at_pos:
+            d.pos = pos
         for entry, descs in self._graph:
             status = entry(handle, *descs)
             if status != 0:
