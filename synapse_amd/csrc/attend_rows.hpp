@@ -32,8 +32,8 @@
 // alone is 2e-4 off in the output. They are scaled by 2^6 (and at most 2^8
 // above that, before the running maximum follows), so that lo is a normal
 // number wherever it counts. With an 8-bit state p carries its key's V step,
-// held against the power of two above the largest step so far (`vexp`), so
-// steps of any size keep that range.
+// held against the power of two above the largest step so far that the row
+// sees (`vexp`), so steps of any size keep that range.
 #pragma once
 
 #include "attend_rows_plan.hpp"
@@ -53,6 +53,7 @@ constexpr float no_max = -3.0e38f;  // before any score (finite: a score of -inf
 
 typedef unsigned int u2 __attribute__((ext_vector_type(2)));
 typedef float f2 __attribute__((ext_vector_type(2)));
+typedef int i2 __attribute__((ext_vector_type(2)));
 
 // Eight bytes (value + 128) as halves, exactly.
 __device__ __forceinline__ h8 bytes_h8(unsigned lo, unsigned hi) {
@@ -135,10 +136,10 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) {
     return l == 0.0f ? 0.0f : l * fast_exp2(m - top);  // (l == 0: nothing seen, m may be -inf)
 }
 
-// The exponent of the power of two above the largest of a tile's V steps
-// (`top`, the same in every lane), or no_vexp.
+// The exponent of the power of two above the largest of a tile's V steps, or
+// no_vexp.
 __device__ __forceinline__ int step_exp(float top) {
-    return __builtin_amdgcn_readfirstlane(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : no_vexp);
+    return top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : no_vexp;
 }
 
 // x / group for x below 2^32 / group (a row of the block, counted from its
@@ -243,7 +244,7 @@ struct wave_rows {
     f2 mref, l;
     h8 hi[RT][2], lo[RT][2];    // the last step's probabilities
     uint32_t seen[RT];          // its keys that the row sees, by score
-    int vexp;
+    i2 vexp;                    // 8-bit states: the exponent that the row's V steps are held against
 
     struct raw_q {
         f4 x[RT][DC][2];
@@ -255,7 +256,7 @@ struct wave_rows {
         col = lane % 16;
         row0 = b.row0 + skip;
         from = b.head0 + skip;
-        vexp = no_vexp;
+        vexp = i2{no_vexp, no_vexp};
         const uint32_t rows = a.n * a.group;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -333,25 +334,32 @@ struct wave_rows {
         }
     }
 
-    // The steps' power of two is now e: what is summed already goes with it.
-    __device__ __forceinline__ void raise_vexp(int e) {
-        if (e > vexp) {
-            const float f = vexp == no_vexp ? 0.0f : ldexpf(1.0f, vexp - e);
+    // Row rt's V steps go up to 2^e: what is summed already goes with them.
+    __device__ __forceinline__ void raise_vexp(int rt, int e) {
+        if (any_lane(e > vexp[rt])) {
+            const int to = e > vexp[rt] ? e : vexp[rt];
+            const float f = vexp[rt] == no_vexp ? 0.0f : ldexpf(1.0f, vexp[rt] - to);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    acc[rt][dt] *= f;
-                }
+            for (int dt = 0; dt < DT; ++dt) {
+                acc[rt][dt] *= f;
             }
-            vexp = e;
+            vexp[rt] = to;
+        }
+    }
+    // The same for a tile that all rows see.
+    __device__ __forceinline__ void raise_vexp(int e) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            raise_vexp(rt, e);
         }
     }
 
     // Scores of the tile at key0 to probabilities, split into hi and lo. ks: the
     // keys' K steps times the scale in exp2's units (or that scale alone); vm:
     // their V steps over 2^vexp. MASKED: some row may not see some of the
-    // tile's keys. While no lane has a score more than `lazy` above its row's
+    // tile's keys; vm are the steps themselves then, and each row's vexp comes
+    // from those that it sees (against a large one that it does not see, its
+    // own would leave the halves' range). While no lane has a score more than `lazy` above its row's
     // maximum, lanes need nothing from each other.
     template <bool MASKED, class KS, class VM>
     __device__ __forceinline__ void softmax(const attend_rows_args& a, const f4 (&s)[RT][4], uint32_t key0, KS ks,
@@ -375,6 +383,14 @@ struct wave_rows {
                 }
             }
             seen[rt] = bits;
+            if constexpr (EIGHT && MASKED) {
+                float top = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    top = fmaxf(top, bits >> j & 1 ? vm(j) : 0.0f);
+                }
+                raise_vexp(rt, step_exp(max32(max16(top))));
+            }
             float p[16];  // over the maximum, in exp2's units
             const auto over = [&](float m) {
 #pragma unroll
@@ -414,14 +430,10 @@ struct wave_rows {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 l[rt] += p[j];
-                if constexpr (EIGHT) {
+                if constexpr (EIGHT && MASKED) {  // a masked key's step may be anything
+                    p[j] = bits >> j & 1 ? p[j] * ldexpf(vm(j), -vexp[rt]) : 0.0f;
+                } else if constexpr (EIGHT) {
                     p[j] *= vm(j);
-                }
-            }
-            if constexpr (EIGHT && MASKED) {  // a masked key's step may be NaN
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    p[j] = bits >> j & 1 ? p[j] : 0.0f;
                 }
             }
 #pragma unroll
@@ -574,11 +586,9 @@ struct wave_rows {
             for (int dt = 0; dt < DT; ++dt) {
                 acc[rt][dt] *= inv;
                 if constexpr (EIGHT) {
-                    if (vexp != no_vexp) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            acc[rt][dt][e] = ldexpf(acc[rt][dt][e], vexp);
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        acc[rt][dt][e] = ldexpf(acc[rt][dt][e], vexp[rt] == no_vexp ? 0 : vexp[rt]);
                     }
                 }
             }
@@ -762,19 +772,21 @@ __global__ __launch_bounds__(256, SRC::eight && DC <= 4 ? 2 : 1) void attend_few
         const uint32_t key0 = tile * attend_tile;
         if constexpr (SRC::eight) {
             float vm[16];
-            float top = 0.0f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 vm[j] = src.vs[j / 4][j % 4];
-                if constexpr (MASKED) {  // past the last key the steps may be anything
-                    vm[j] = key0 + score_key(j, rows.G) < b.len ? vm[j] : 0.0f;
-                }
-                top = fmaxf(top, vm[j]);
             }
-            rows.raise_vexp(step_exp(max32(max16(top))));
+            if constexpr (!MASKED) {
+                float top = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                vm[j] = ldexpf(vm[j], -rows.vexp);
+                for (int j = 0; j < 16; ++j) {
+                    top = fmaxf(top, vm[j]);
+                }
+                rows.raise_vexp(step_exp(max32(max16(top))));
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    vm[j] = ldexpf(vm[j], -rows.vexp[0]);
+                }
             }
             rows.template softmax<MASKED>(a, s, key0, [&](int j) { return src.ks[j / 4][j % 4] * a.scale_log2e; },
                                           [&](int j) { return vm[j]; });
@@ -878,7 +890,8 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
     const _Float16* vh = EIGHT ? nullptr : a.vt + size_t{b.g} * a.hd * a.ctx_stride;
     u4 next[COPY ? 1 : LOADS];
     float next_ks = 0.0f, next_vs = 0.0f;
-    int run_vexp = no_vexp;  // wave 0's: the steps' power of two up to the staged tile
+    int run_vexp = no_vexp;  // wave 0's: the power of two of the steps staged for all rows
+    const uint32_t whole = max(b.t_begin, min(b.t_end, open / attend_tile));  // from here on tiles are masked
 
     // A tile's loads into registers, or (binary16) copies to buffer buf.
     const auto load = [&](uint32_t tile, uint32_t buf) {
@@ -950,13 +963,13 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
                 to[at + then] = bytes_h8(next[i][2], next[i][3]);
             }
             if (w == 0) {
-                const bool in = tile * attend_tile + lane < b.len;  // past the last key the steps may be anything
-                next_ks = in ? next_ks : 0.0f;
-                next_vs = in ? next_vs : 0.0f;
-                const int e = step_exp(wave_reduce_max(next_vs));
-                run_vexp = e > run_vexp ? e : run_vexp;
+                if (tile < whole) {
+                    const int e = step_exp(wave_reduce_max(next_vs));
+                    run_vexp = e > run_vexp ? e : run_vexp;
+                    next_vs = ldexpf(next_vs, -run_vexp);
+                }
                 ks_lds[buf][lane] = next_ks * a.scale_log2e;
-                vs_lds[buf][lane] = ldexpf(next_vs, -run_vexp);
+                vs_lds[buf][lane] = next_vs;
                 if (lane == 0) {
                     vexp_lds[buf] = run_vexp;
                 }
@@ -983,7 +996,9 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
         f4 s[RT][4];
         rows.template stream_k<4>(from, s, k_in);
         if constexpr (EIGHT) {
-            rows.raise_vexp(__builtin_amdgcn_readfirstlane(vexp_lds[buf]));
+            if constexpr (!MASKED) {
+                rows.raise_vexp(__builtin_amdgcn_readfirstlane(vexp_lds[buf]));
+            }
             f4 ks[4], vm[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -1019,7 +1034,6 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
             __syncthreads();
         }
     };
-    const uint32_t whole = max(b.t_begin, min(b.t_end, open / attend_tile));
     run(b.t_begin, whole, std::false_type{});
     run(whole, b.t_end, std::true_type{});
 
@@ -1069,7 +1083,8 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
     const _Float16* vh = EIGHT ? nullptr : a.vt + size_t{b.g} * a.hd * a.ctx_stride;
     u4 next[LOADS];
     float next_ks = 0.0f, next_vs = 0.0f;
-    int run_vexp = no_vexp;  // wave 4's: the steps' power of two up to the staged tile
+    int run_vexp = no_vexp;  // wave 4's: the power of two of the steps staged for all rows
+    const uint32_t whole = max(b.t_begin, min(b.t_end, open / attend_tile));  // from here on tiles are masked
 
     // This group's part (K or V) of a tile: 8-bit loads into registers, to be
     // staged; binary16 copies straight to their buffer.
@@ -1133,12 +1148,14 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
     };
     const auto stage_steps = [&](uint32_t tile) {
         if (EIGHT && w == 4 && tile < b.t_end) {
-            const bool in = tile * attend_tile + lane < b.len;  // past the last key the steps may be anything
-            const float ks = in ? next_ks : 0.0f, vs = in ? next_vs : 0.0f;
-            const int e = step_exp(wave_reduce_max(vs));
-            run_vexp = e > run_vexp ? e : run_vexp;
-            ks_lds[tile & 1][lane] = ks * a.scale_log2e;
-            vs_lds[tile & 1][lane] = ldexpf(vs, -run_vexp);
+            float vs = next_vs;
+            if (tile < whole) {
+                const int e = step_exp(wave_reduce_max(vs));
+                run_vexp = e > run_vexp ? e : run_vexp;
+                vs = ldexpf(vs, -run_vexp);
+            }
+            ks_lds[tile & 1][lane] = next_ks * a.scale_log2e;
+            vs_lds[tile & 1][lane] = vs;
             if (lane == 0) {
                 vexp_lds[tile & 1] = run_vexp;
             }
@@ -1202,7 +1219,9 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
                 }
                 if (key0 < reach) {
                     if constexpr (EIGHT) {
-                        rows.raise_vexp(__builtin_amdgcn_readfirstlane(vexp));
+                        if constexpr (!MASKED) {
+                            rows.raise_vexp(__builtin_amdgcn_readfirstlane(vexp));
+                        }
                         rows.template softmax<MASKED>(a, s, key0, [&](int j) { return ks[j / 4][j % 4]; },
                                                       [&](int j) { return vm[j / 4][j % 4]; });
                     } else {
@@ -1237,7 +1256,6 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
                 turn();
             }
         };
-        const uint32_t whole = max(t0, min(t1, open / attend_tile));
         run(t0, whole, std::false_type{});
         run(whole, t1, std::true_type{});
         if (k_group) {

@@ -219,6 +219,98 @@ def test_causal_run_with_wild_rows_8bit(room):
     assert_held(attend8(room, cache, q, 0, n_heads, 0.2), want, tol)
 
 
+# (query heads, KV heads, head size, tokens): up to 16 rows a KV head, 64, 128, and more.
+ROW_COUNTS = [(2, 1, 64, 8), (4, 2, 64, 30), (8, 2, 64, 29), (8, 2, 64, 45), (8, 2, 96, 75), (8, 2, 160, 45), (4, 1, 18, 45)]
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,n", ROW_COUNTS)
+@pytest.mark.parametrize("pos,tree", [(0, False), (40, False), (40, True), (100, True)])
+def test_larger_steps_of_unseen_keys(room, n_heads, n_kv, hd, n, pos, tree):
+    """V rows that grow from token to token, by 2^160 in all: each token's
+    output is right to the values it sees itself, however much larger those
+    are that it does not see."""
+    g = np.random.default_rng(pos + n)
+    x = g.standard_normal((2, pos + n, n_kv, hd)).astype(np.float32)
+    x[1, pos:] *= (2.0 ** np.linspace(-80, 80, n)).astype(np.float32)[:, None, None]
+    x[1, :pos] *= np.float32(2.0 ** -80)
+    cache = capi.kv8_state(room, pos + n + 3, n_kv, hd)
+    append8(room, cache, x[0], x[1], 0)
+    q = g.standard_normal((n, n_heads * hd)).astype(np.float32)
+    mask = random_tree(g, n) if tree else None
+    sees = tree_sees(mask, n, pos) if tree else causal(n, pos)
+    want, tol = attend64(q, values(x[0]), values(x[1]), n_heads, 0.125, sees)
+    got = attend8(room, cache, q, pos, n_heads, 0.125, mask=mask)
+    for i in range(n):
+        assert_held(got[i:i + 1], want[i:i + 1], tol[i:i + 1], f"token {i}")
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,n", ROW_COUNTS)
+@pytest.mark.parametrize("eight", [False, True])
+def test_wild_rows_at_every_row_count(room, n_heads, n_kv, hd, n, eight):
+    """Infinities and NaN in drafted K and V rows, in a tile that ends inside
+    the state and one that does not; what lies behind the rows is NaN too."""
+    pos = 57
+    g = np.random.default_rng(n + hd)
+    x = g.standard_normal((2, pos + n, n_kv, hd)).astype(np.float32)
+    for j, bad in ((2, np.inf), (3, -np.inf), (5, np.nan), (n - 1, np.inf)):
+        x[1, pos + j, 0, j % hd] = bad
+    x[0, pos + 4, n_kv - 1, 1] = np.nan
+    if eight:
+        cache = capi.kv8_state(room, pos + n + 70, n_kv, hd)
+        append8(room, cache, x[0], x[1], 0)
+        k, v = values(x[0]), values(x[1])
+    else:
+        cache, k, v = _state16(room, g, pos + n, pos + n + 70, n_kv, hd)
+        rows = x.astype(np.float16)
+        kc = np.full((cache.max_ctx, n_kv * hd), 0x7e00, np.uint16)
+        vt = np.full((n_kv * hd, cache.ctx_stride), 0x7c00, np.uint16)
+        kc[:pos + n] = rows[0].reshape(pos + n, -1).view(np.uint16)
+        vt[:, :pos + n] = rows[1].reshape(pos + n, -1).view(np.uint16).T
+        room.upload(cache.k_offset, kc)
+        room.upload(cache.v_offset, vt)
+        k, v = rows.astype(np.float64)
+    q = g.standard_normal((n, n_heads * hd)).astype(np.float32)
+    mask = capi.tree_mask([int(g.integers(max(-1, i - 4), i)) for i in range(n)])
+    want, tol = attend64(q, k, v, n_heads, 0.125, tree_sees(mask, n, pos))
+    got = attend8(room, cache, q, pos, n_heads, 0.125, mask=mask) if eight else \
+        attend_tree(room, cache, q, pos, n_heads, 0.125, mask)
+    assert np.isfinite(want).any() and not np.isfinite(want).all()
+    assert_held(got, want, tol)
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,n", ROW_COUNTS)
+@pytest.mark.parametrize("eight", [False, True])
+def test_tree_of_binary16_queries(room, n_heads, n_kv, hd, n, eight):
+    g = np.random.default_rng(n)
+    pos = 190
+    cache, k, v = (_state8 if eight else _state16)(room, g, pos + n, pos + n, n_kv, hd)
+    q = g.standard_normal((n, n_heads * hd)).astype(np.float16)
+    mask = random_tree(g, n)
+    want, tol = attend64(q, k, v, n_heads, 0.125, tree_sees(mask, n, pos))
+    got = attend8(room, cache, q, pos, n_heads, 0.125, mask=mask, q_dtype=SYN_F16) if eight else \
+        attend_tree(room, cache, q, pos, n_heads, 0.125, mask, q_dtype=SYN_F16)
+    assert_held(got, want, tol)
+
+
+@pytest.mark.parametrize("pos", [0, 63, 64, 500])
+@pytest.mark.parametrize("kv_dtype", [SYN_F32, SYN_F16])
+def test_append_and_attend_in_one_call(room, pos, kv_dtype):
+    """syn_hip_kv8_attention for one token and for a run, against its two halves."""
+    n_heads, n_kv, hd = 8, 2, 128
+    g = np.random.default_rng(pos)
+    for n in (1, 40):
+        x = g.standard_normal((2, pos + n, n_kv, hd)).astype(np.float16 if kv_dtype == SYN_F16 else np.float32)
+        one, two = (capi.kv8_state(room, pos + n, n_kv, hd) for _ in range(2))
+        q = g.standard_normal((n, n_heads * hd)).astype(np.float32)
+        append8(room, two, x[0], x[1], 0, kv_dtype)
+        if pos:
+            append8(room, one, x[0, :pos], x[1, :pos], 0, kv_dtype)
+        got = attend8(room, one, q, pos, n_heads, 0.1, rows=(x[0, pos:], x[1, pos:]), kv_dtype=kv_dtype)
+        assert np.array_equal(got, attend8(room, two, q, pos, n_heads, 0.1))
+        for a, b in zip(read8(room, one, pos + n, 0), read8(room, two, pos + n, 0)):
+            assert np.array_equal(a, b)
+
+
 def test_a_chain_is_a_causal_run(room):
     """A tree with one branch equals the framework's causal attention to that
     kernel's binary16 probabilities (2^-11 each way), and kv8_attend's own."""
