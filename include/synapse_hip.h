@@ -170,8 +170,8 @@ int syn_hip_attend_batch(syn_arena* arena, const syn_seq_desc* seqs, uint32_t n_
  * half the size: each row (position, KV head) of K and of V is head_dim
  * whole numbers q in -127..127 and one f32 step d,
  *   d = max|x| / 127 (rounded to f32),  q = x / d to the nearest whole
- * number, ties to even, and stands for the values q * d. A row of zeros has
- * step 0; a row with an infinity or NaN stands for NaN throughout, and makes
+ * number, ties to even, and stands for the values q * d. A row of zeros (or
+ * of values so small that d rounds to 0) has step 0; a row with an infinity or NaN stands for NaN throughout, and makes
  * NaN of the outputs that attend it and of no others. The bytes' order in
  * the arena is the library's own; nothing in a state needs to start at
  * zero. Positions, heads and limits as for syn_kv_desc, with max_ctx at most
@@ -224,7 +224,8 @@ typedef struct syn_kv8_attn_desc {
 /* Scratch for calls of up to max_batch tokens on a state of max_ctx. */
 uint64_t syn_hip_kv8_attention_scratch_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
                                              uint32_t max_ctx, uint32_t max_batch);
-/* Appends the run's n rows, then attends (syn_hip_attention's two halves), */
+/* Appends the run's n rows, then attends (syn_hip_attention's two halves);
+ * none of q, the rows and the mask may overlap the state: */
 int syn_hip_kv8_attention(syn_arena* arena, const syn_kv8_attn_desc* desc);
 /* or attends only: positions 0..pos+n-1 are in the state (k_offset and
  * v_offset are ignored). */

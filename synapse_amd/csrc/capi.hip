@@ -1619,6 +1619,12 @@ int syn_hip_kv8_attention(syn_arena* a, const syn_kv8_attn_desc* d) {
     if (int e = fill_kv8_attend(a, d, r)) {  // before the append: a refused call changes nothing
         return e;
     }
+    const uint64_t q_bytes = uint64_t{d->n} * d->n_heads * d->cache.head_dim * dtype_size(d->q_dtype);
+    const uint64_t mask_bytes = r.mask != nullptr ? uint64_t{d->n} * r.mask_words * 4 : 0;
+    if (int e = check_apart("kv8 attention", {kv8_span(d->cache)},
+                            {{d->q_offset, q_bytes, "q"}, {d->mask_offset, mask_bytes, "the mask"}})) {
+        return e;
+    }
     if (int e = syn_hip_kv8_append(a, &d->cache, d->k_offset, d->v_offset, d->n, d->pos, d->kv_dtype)) {
         return e;
     }

@@ -70,6 +70,9 @@ def refusals() -> list:
         if eight:
             add(f"{what}: mask off 4", EINVAL, fn, _copy(d, mask_offset=3 * MIB + 2))
             add(f"{what}: mask past the arena", ERANGE, fn, _copy(d, mask_offset=32 * MIB - 16))
+            if fn is L.syn_hip_kv8_attention:  # (it writes the state before it reads these)
+                add(f"{what}: q in the state", EINVAL, fn, _copy(d, q_offset=1024))
+                add(f"{what}: mask in the state", EINVAL, fn, _copy(d, mask_offset=1024))
             add(f"{what}: mask in the output", EINVAL, fn, _copy(d, mask_offset=7 * MIB))
             add(f"{what}: state off 256", EINVAL, fn, _copy(d, cache=_copy(state, offset=16)))
             add(f"{what}: state past the arena", ERANGE, fn, _copy(d, cache=_copy(state, offset=32 * MIB - 256)))
