@@ -119,16 +119,28 @@ __device__ __forceinline__ h8 k_halves(const _Float16* p, uint32_t d, uint32_t h
     }
 }
 
-// Bits 0..7 of draft row `bits` from drafted token j on (j may start before
-// the first or end past the last): whole words in range, so no read is
-// outside the row's `words` words.
-__device__ __forceinline__ uint32_t mask_bits8(const uint32_t* bits, uint32_t words, uint32_t n, int j) {
-    const int w = j >> 5;  // rounds down
-    const uint32_t lo = w >= 0 && w < static_cast<int>(words) ? bits[w] : 0u;
-    const uint32_t hi = w + 1 >= 0 && w + 1 < static_cast<int>(words) ? bits[w + 1] : 0u;
-    const uint64_t both = (uint64_t{hi} << 32 | lo) >> (j & 31);
-    const int left = static_cast<int>(n) - j;  // bits past the last token are ignored
-    return static_cast<uint32_t>(both) & (left >= 8 ? 0xffu : left > 0 ? (1u << left) - 1u : 0u);
+// Of eight keys of a binary16 V^T row, the first `left` (all ones for theirs).
+__device__ __forceinline__ u4 first_halves(uint32_t left) {
+    u4 keep;
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+        keep[e] = left >= 2 * e + 2 ? 0xffffffffu : left == 2 * e + 1 ? 0xffffu : 0u;
+    }
+    return keep;
+}
+// The larger magnitudes of x's halves and top's, as bits.
+__device__ __forceinline__ uint32_t top_halves(uint32_t top, u4 x) {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t y = x[e] & 0x7fff7fffu;
+        top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, top), __builtin_bit_cast(us2, y)));
+    }
+    return top;
+}
+// Whether one of them is infinite or NaN.
+__device__ __forceinline__ bool wild_halves(uint32_t top) {
+    return (top & 0xffffu) >= 0x7c00u || top >> 16 >= 0x7c00u;
 }
 
 // Weight of a part (max, sum) of a row whose maximum is top.
@@ -234,8 +246,6 @@ struct wave_rows {
     static_assert(RT <= 2);
     uint32_t G, col, row0;
     uint32_t from;              // row0, counted from the first head of the block's first token
-    uint32_t limit[RT];         // keys seen without the mask (0: no row)
-    const uint32_t* draft[RT];  // the row's mask
     h8 q[RT][DC];
     f4 acc[RT][DT];             // O^T: dims 16 dt + 4 G .. + 3
     // The running maximum less p_shift; the sum of this lane's keys. Vectors:
@@ -243,29 +253,21 @@ struct wave_rows {
     // place read the dispatch packet in host memory (1 to 13 us of a start).
     f2 mref, l;
     h8 hi[RT][2], lo[RT][2];    // the last step's probabilities
-    uint32_t seen[RT];          // its keys that the row sees, by score
+    uint32_t seen[RT];          // the keys of a masked tile that the row sees, by score
     i2 vexp;                    // 8-bit states: the exponent that the row's V steps are held against
 
     struct raw_q {
         f4 x[RT][DC][2];
     };
     // Rows from row `skip` of the block's on.
-    __device__ __forceinline__ void place(const attend_rows_args& a, const block_place& b, uint32_t skip,
-                                          uint32_t lane) {
+    __device__ __forceinline__ void place(const block_place& b, uint32_t skip, uint32_t lane) {
         G = lane / 16;
         col = lane % 16;
         row0 = b.row0 + skip;
         from = b.head0 + skip;
         vexp = i2{no_vexp, no_vexp};
-        const uint32_t rows = a.n * a.group;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const bool in = row0 + rt * 16 + col < rows;
-            const uint32_t token = in ? b.token0 + div_group(a, from + rt * 16 + col) : 0;
-            limit[rt] = !in ? 0 : TREE ? a.pos : a.pos + token + 1;
-            if constexpr (TREE) {
-                draft[rt] = a.mask + size_t{token} * a.mask_words;
-            }
             mref[rt] = no_max;
             l[rt] = 0.0f;
 #pragma unroll
@@ -354,35 +356,62 @@ struct wave_rows {
         }
     }
 
+    // Which keys of the tile at key0 the rows see. A lane's two eights of keys,
+    // 32 apart, lie in three words of its row's mask, loaded without branches
+    // (with them each was waited for before the next: 4 us a tile), words
+    // outside the row from its first. Rows' tokens and limits are found again
+    // for each of the few masked tiles: kept, they took the other tiles'
+    // registers (a tree of 61: 50 us, 46).
+    __device__ __forceinline__ void take_mask(const attend_rows_args& a, const block_place& b, uint32_t key0) {
+        const int w = static_cast<int>(key0 + G * 8 - a.pos) >> 5, words = static_cast<int>(a.mask_words);
+        uint32_t word[RT][3];
+        if constexpr (TREE) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const bool in = row0 + rt * 16 + col < a.n * a.group;
+                const uint32_t token = in ? b.token0 + div_group(a, from + rt * 16 + col) : 0;
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    word[rt][i] = a.mask[size_t{token} * a.mask_words + (w + i >= 0 && w + i < words ? w + i : 0)];
+                }
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const bool in = row0 + rt * 16 + col < a.n * a.group;
+            const uint32_t all = !in ? 0 : TREE ? a.pos : a.pos + b.token0 + div_group(a, from + rt * 16 + col) + 1;
+            uint32_t bits = 0;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const uint32_t k0 = key0 + score_key(8 * c, G);
+                const uint32_t open = all > k0 ? all - k0 : 0;
+                uint32_t eight = open >= 8 ? 0xffu : (1u << open) - 1u;
+                if constexpr (TREE) {
+                    const int j = static_cast<int>(k0 - a.pos);  // (the first before or behind the drafted tokens: none)
+                    const uint32_t lo = w + c >= 0 && w + c < words ? word[rt][c] : 0u;
+                    const uint32_t hi = w + c + 1 >= 0 && w + c + 1 < words ? word[rt][c + 1] : 0u;
+                    const uint32_t drafted = static_cast<uint32_t>((uint64_t{hi} << 32 | lo) >> (j & 31));
+                    const int left = static_cast<int>(a.n) - j;  // bits past the last token are ignored
+                    eight |= in ? drafted & (left >= 8 ? 0xffu : left > 0 ? (1u << left) - 1u : 0u) : 0u;
+                }
+                bits |= eight << (8 * c);
+            }
+            seen[rt] = bits;
+        }
+    }
+
     // Scores of the tile at key0 to probabilities, split into hi and lo. ks: the
     // keys' K steps times the scale in exp2's units (or that scale alone); vm:
     // their V steps over 2^vexp. MASKED: some row may not see some of the
-    // tile's keys; vm are the steps themselves then, and each row's vexp comes
-    // from those that it sees (against a large one that it does not see, its
+    // tile's keys (take_mask); vm are the steps themselves then, and each row's
+    // vexp comes from those that it sees (against a large one that it does not see, its
     // own would leave the halves' range). While no lane has a score more than `lazy` above its row's
     // maximum, lanes need nothing from each other.
     template <bool MASKED, class KS, class VM>
-    __device__ __forceinline__ void softmax(const attend_rows_args& a, const f4 (&s)[RT][4], uint32_t key0, KS ks,
-                                            VM vm) {
+    __device__ __forceinline__ void softmax(const f4 (&s)[RT][4], KS ks, VM vm) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            uint32_t bits = 0xffffu;
-            if constexpr (MASKED) {
-                bits = 0;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const uint32_t k0 = key0 + score_key(8 * c, G);
-                    const uint32_t left = limit[rt] > k0 ? limit[rt] - k0 : 0;
-                    uint32_t b = left >= 8 ? 0xffu : (1u << left) - 1u;
-                    if constexpr (TREE) {
-                        if (row0 + rt * 16 + col < a.n * a.group) {
-                            b |= mask_bits8(draft[rt], a.mask_words, a.n, static_cast<int>(k0 - a.pos));
-                        }
-                    }
-                    bits |= b << (8 * c);
-                }
-            }
-            seen[rt] = bits;
+            const uint32_t bits = MASKED ? seen[rt] : 0xffffu;
             if constexpr (EIGHT && MASKED) {
                 float top = 0.0f;
 #pragma unroll
@@ -520,34 +549,26 @@ struct wave_rows {
             acc[rt][dt] = mfma16(v, lo[rt][c], acc[rt][dt]);
         }
     }
-    // The same in a tile of a binary16 state that holds drafted rows, or ends
-    // before its end: of v's keys the first `left` are there, and a value that
-    // is infinite or NaN, which as an operand would reach the rows that do not
-    // see it (0 times it is NaN), gets products of its own: a row has +inf
-    // added where it sees a +inf or NaN among the 32 keys, and -inf where it
-    // sees a -inf or NaN (so NaN where both).
-    __device__ __forceinline__ void add_v_tail(int dt, int c, h8 v, uint32_t left) {
-        h8 finite;
+    // The same in a masked tile of a binary16 state that holds infinities or
+    // NaN, which as an operand would reach the rows that do not see them (0
+    // times one is NaN). They get products of their own: a row has +inf added
+    // where it sees a +inf or NaN among the 32 keys, and -inf where it sees a
+    // -inf or NaN (so NaN where both).
+    __device__ __forceinline__ void add_wild_v(int dt, int c, h8 v) {
+        h8 finite, up, down;
         bool any = false;
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) {
             const _Float16 x = v[e];  // (a bit cast of the element itself casts element 0)
             const unsigned short b = __builtin_bit_cast(unsigned short, x);
-            const bool wild = (b & 0x7c00u) == 0x7c00u;
-            finite[e] = e < left && !wild ? x : static_cast<_Float16>(0);
-            any = any || (e < left && wild);
+            const bool wild = (b & 0x7c00u) == 0x7c00u, nan = (b & 0x3ffu) != 0;
+            finite[e] = wild ? static_cast<_Float16>(0) : x;
+            up[e] = static_cast<_Float16>(wild && (nan || b >> 15 == 0) ? 1.0f : 0.0f);
+            down[e] = static_cast<_Float16>(wild && (nan || b >> 15 != 0) ? 1.0f : 0.0f);
+            any = any || wild;
         }
         add_v(dt, c, finite);
         if (any_lane(any)) {
-            h8 up, down;
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) {
-                const _Float16 x = v[e];
-                const unsigned short b = __builtin_bit_cast(unsigned short, x);
-                const bool wild = e < left && (b & 0x7c00u) == 0x7c00u, nan = (b & 0x3ffu) != 0;
-                up[e] = static_cast<_Float16>(wild && (nan || b >> 15 == 0) ? 1.0f : 0.0f);
-                down[e] = static_cast<_Float16>(wild && (nan || b >> 15 != 0) ? 1.0f : 0.0f);
-            }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 h8 sees;
@@ -564,14 +585,14 @@ struct wave_rows {
             }
         }
     }
-
-    __device__ __forceinline__ void add_tail(const h8* v_from, uint32_t key0, uint32_t len) {
+    template <class V>
+    __device__ __forceinline__ void add_wild(V v) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const uint32_t key = key0 + score_key(8 * c, G);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                add_v_tail(dt, c, v_from[(dt * 2 + c) * 64], len > key ? len - key : 0);
+                add_wild_v(dt, c, v(dt, c));
+                __builtin_amdgcn_sched_barrier(0);  // (the next operand's read would take registers)
             }
         }
     }
@@ -626,6 +647,27 @@ struct wave_rows {
         }
     }
 };
+
+// A wave's V operands of a masked tile (every fourth), in LDS: keys past the
+// last one to zeros (what is there could be NaN). Whether some of the rest is
+// infinite or NaN.
+template <int DC>
+__device__ __forceinline__ bool clean_v(h8* v, uint32_t w, uint32_t lane, uint32_t tile, uint32_t len) {
+    uint32_t top = 0;
+    const uint32_t key = tile * attend_tile + w % 2 * 32 + lane / 16 * 8;  // (operand 2 dt + c, w and c of one parity)
+    const u4 keep = first_halves(len > key ? len - key : 0);
+#pragma unroll
+    for (int i = 0; i < DC; ++i) {
+        h8* at = v + (i * 4 + w) * 64 + lane;
+        const u4 x = as_u4(*at) & keep;
+        top = top_halves(top, x);
+        *at = as_h8(x);
+    }
+    return any_lane(wild_halves(top));
+}
+__device__ __forceinline__ bool any_wild(const int (&wild)[attend_waves]) {
+    return __builtin_amdgcn_readfirstlane(wild[0] | wild[1] | wild[2] | wild[3]) != 0;
+}
 
 // ---- up to 16 rows: each wave its own tiles, from memory to operands ---------
 template <int DC>
@@ -721,6 +763,23 @@ struct f16_source {
             }
         }
     }
+    // V past the last key to zeros (what is there could be NaN); whether some
+    // of the rest is infinite or NaN.
+    __device__ __forceinline__ bool clean(uint32_t tile, uint32_t lane) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const uint32_t key = tile * attend_tile + c * 32 + lane / 16 * 8;
+            const u4 keep = first_halves(len > key ? len - key : 0);
+#pragma unroll
+            for (int dt = 0; dt < 2 * DC; ++dt) {
+                const u4 x = as_u4(vq[dt][c]) & keep;
+                top = top_halves(top, x);
+                vq[dt][c] = as_h8(x);
+            }
+        }
+        return any_lane(wild_halves(top));
+    }
     __device__ __forceinline__ h8 k(int st, int dc) const {
         return kq[st][dc];
     }
@@ -749,7 +808,7 @@ __global__ __launch_bounds__(256, SRC::eight && DC <= 4 ? 2 : 1) void attend_few
 
     wave_rows<DC, 1, SRC::eight, TREE> rows;
     typename decltype(rows)::raw_q raw;
-    rows.place(a, b, 0, lane);
+    rows.place(b, 0, lane);
     rows.load_q(a, b, raw);
     SRC src(a, b.g, b.len);
     uint32_t tile = b.t_begin + w;
@@ -769,7 +828,9 @@ __global__ __launch_bounds__(256, SRC::eight && DC <= 4 ? 2 : 1) void attend_few
                 s[0][st] = mfma16(src.k(st, dc), rows.q[0][dc], s[0][st]);
             }
         }
-        const uint32_t key0 = tile * attend_tile;
+        if constexpr (MASKED) {
+            rows.take_mask(a, b, tile * attend_tile);
+        }
         if constexpr (SRC::eight) {
             float vm[16];
 #pragma unroll
@@ -788,19 +849,24 @@ __global__ __launch_bounds__(256, SRC::eight && DC <= 4 ? 2 : 1) void attend_few
                     vm[j] = ldexpf(vm[j], -rows.vexp[0]);
                 }
             }
-            rows.template softmax<MASKED>(a, s, key0, [&](int j) { return src.ks[j / 4][j % 4] * a.scale_log2e; },
+            rows.template softmax<MASKED>(s, [&](int j) { return src.ks[j / 4][j % 4] * a.scale_log2e; },
                                           [&](int j) { return vm[j]; });
         } else {
-            rows.template softmax<MASKED>(a, s, key0, [&](int) { return a.scale_log2e; }, [](int) { return 1.0f; });
+            rows.template softmax<MASKED>(s, [&](int) { return a.scale_log2e; }, [](int) { return 1.0f; });
         }
+        bool wild = false;
+        if constexpr (!SRC::eight) {
+            if constexpr (MASKED) {
+                wild = src.clean(tile, lane);
+            }
+        }
+        if (wild) {
+            rows.add_wild([&](int dt, int c) { return src.v(dt, c); });
+        } else {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const uint32_t key = key0 + score_key(8 * c, rows.G);
+            for (int c = 0; c < 2; ++c) {
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                if constexpr (!SRC::eight && MASKED) {
-                    rows.add_v_tail(dt, c, src.v(dt, c), b.len > key ? b.len - key : 0);
-                } else {
+                for (int dt = 0; dt < DT; ++dt) {
                     rows.add_v(dt, c, src.v(dt, c));
                 }
             }
@@ -872,6 +938,7 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
     __shared__ h8 tiles[2][8 * DC][64];
     __shared__ float ks_lds[2][attend_tile], vs_lds[2][attend_tile];
     __shared__ int vexp_lds[2];
+    __shared__ int wild_lds[2][attend_waves];
 
     const uint32_t lane = threadIdx.x % 64;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -942,6 +1009,14 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
                 to[(i * 4 + w) * 64 + lane] = as_h8(next[i]);
                 to[(v_frag + i * 4 + w) * 64 + lane] = as_h8(next[DC + i]);
             }
+        }
+        if constexpr (!EIGHT) {
+            if (tile >= whole) {
+                const bool wild = clean_v<DC>(&tiles[buf][v_frag][0], w, lane, tile, b.len);
+                if (lane == 0) {
+                    wild_lds[buf][w] = wild;
+                }
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
@@ -980,7 +1055,7 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
     wave_rows<DC, RT, EIGHT, TREE> rows;
     {
         typename decltype(rows)::raw_q raw;
-        rows.place(a, b, w * (RT * 16), lane);
+        rows.place(b, w * (RT * 16), lane);
         rows.load_q(a, b, raw);
         if (b.t_begin < b.t_end) {
             load(b.t_begin, 0);
@@ -990,7 +1065,7 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
     }
     __syncthreads();
     const bool k_in = !COPY || (DC - 1) * 32 + rows.G * 8 < a.hd;
-    const auto step = [&](uint32_t key0, uint32_t buf, auto masked) {
+    const auto step = [&](uint32_t buf, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
         const h8* from = &tiles[buf][0][lane];
         f4 s[RT][4];
@@ -1005,13 +1080,13 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
                 ks[j] = *reinterpret_cast<const f4*>(&ks_lds[buf][score_key(4 * j, rows.G)]);
                 vm[j] = *reinterpret_cast<const f4*>(&vs_lds[buf][score_key(4 * j, rows.G)]);
             }
-            rows.template softmax<MASKED>(a, s, key0, [&](int j) { return ks[j / 4][j % 4]; },
+            rows.template softmax<MASKED>(s, [&](int j) { return ks[j / 4][j % 4]; },
                                           [&](int j) { return vm[j / 4][j % 4]; });
         } else {
-            rows.template softmax<MASKED>(a, s, key0, [&](int) { return a.scale_log2e; }, [](int) { return 1.0f; });
+            rows.template softmax<MASKED>(s, [&](int) { return a.scale_log2e; }, [](int) { return 1.0f; });
         }
-        if constexpr (!EIGHT && MASKED) {
-            rows.add_tail(from + v_frag * 64, key0, b.len);
+        if (!EIGHT && MASKED && any_wild(wild_lds[buf])) {
+            rows.add_wild([&](int dt, int c) { return from[(v_frag + dt * 2 + c) * 64]; });
         } else {
             rows.template stream_v<4>(from + v_frag * 64);
         }
@@ -1022,11 +1097,14 @@ __global__ __launch_bounds__(256, DC <= 4 ? 2 : 1) void attend_many_kernel(const
         for (uint32_t tile = from; tile < to; ++tile) {
             const uint32_t buf = (tile - b.t_begin) & 1;
             const bool more = tile + 1 < b.t_end;
+            if (masked.value) {  // (before the next loads: a wait for the words would wait for those too)
+                rows.take_mask(a, b, tile * attend_tile);
+            }
             if (more) {
                 load(tile + 1, buf ^ 1);
             }
             if (tile * attend_tile < reach) {
-                step(tile * attend_tile, buf, masked);
+                step(buf, masked);
             }
             if (more) {
                 stage(tile + 1, buf ^ 1);
@@ -1065,6 +1143,7 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
     __shared__ h8 k_lds[2][4 * DC][64], v_lds[2][4 * DC][64];
     __shared__ float ks_lds[2][attend_tile], vs_lds[2][attend_tile];
     __shared__ int vexp_lds[2];
+    __shared__ int wild_lds[2][attend_waves];  // with V
 
     const uint32_t lane = threadIdx.x % 64, in_group = threadIdx.x % 256;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -1137,6 +1216,12 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
             }
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (!k_group && tile >= whole) {
+                const bool wild = clean_v<DC>(&v_lds[tile & 1][0][0], w % 4, lane, tile, b.len);
+                if (lane == 0) {
+                    wild_lds[tile & 1][w % 4] = wild;
+                }
+            }
         }
     };
     const auto load_steps = [&](uint32_t tile) {
@@ -1168,7 +1253,7 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
     };
 
     wave_rows_t rows;
-    rows.place(a, b, w * (RT * 16), lane);
+    rows.place(b, w * (RT * 16), lane);
     f4 s[RT][4];
     f4 ks[4], vm[4];  // the steps of this lane's keys in the next softmax's tile
     int vexp = no_vexp;
@@ -1214,6 +1299,9 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
             for (uint32_t tile = from; tile < to; ++tile) {
                 const uint32_t key0 = tile * attend_tile;
                 const bool more = tile + 1 < t1;
+                if (MASKED) {  // (before the next loads: a wait for the words would wait for those too)
+                    rows.take_mask(a, b, key0);
+                }
                 if (!EIGHT && more) {
                     load(tile + 1);
                 }
@@ -1222,10 +1310,10 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
                         if constexpr (!MASKED) {
                             rows.raise_vexp(__builtin_amdgcn_readfirstlane(vexp));
                         }
-                        rows.template softmax<MASKED>(a, s, key0, [&](int j) { return ks[j / 4][j % 4]; },
+                        rows.template softmax<MASKED>(s, [&](int j) { return ks[j / 4][j % 4]; },
                                                       [&](int j) { return vm[j / 4][j % 4]; });
                     } else {
-                        rows.template softmax<MASKED>(a, s, key0, [&](int) { return a.scale_log2e; },
+                        rows.template softmax<MASKED>(s, [&](int) { return a.scale_log2e; },
                                                       [](int) { return 1.0f; });
                     }
                 }
@@ -1240,8 +1328,8 @@ __global__ __launch_bounds__(512, 2) void attend_turns_kernel(const attend_rows_
                 if (key0 < reach) {  // (behind the last tile the scores are not used)
                     const h8* v_from = &v_lds[tile & 1][0][lane];
                     const h8* k_from = &k_lds[(tile + 1) & 1][0][lane];
-                    if constexpr (!EIGHT && MASKED) {
-                        rows.add_tail(v_from, key0, b.len);
+                    if (!EIGHT && MASKED && any_wild(wild_lds[tile & 1])) {
+                        rows.add_wild([&](int dt, int c) { return v_from[(dt * 2 + c) * 64]; });
                         rows.template stream_k<4>(k_from, s, k_in);
                     } else {
                         rows.template stream_vk<6>(v_from, k_from, s, k_in);
