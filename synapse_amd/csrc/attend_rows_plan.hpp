@@ -69,7 +69,8 @@ constexpr uint32_t attend_tile = 64;        // keys of a step
 constexpr uint32_t attend_waves = 4;        // waves of a block
 constexpr uint32_t attend_max_splits = 256;
 // Splits are added up to this many waves: two on each of 256 CUs' four SIMDs.
-constexpr uint32_t attend_split_waves = 2048;
+constexpr uint32_t attend_cus = 256;
+constexpr uint32_t attend_split_waves = attend_cus * 4 * 2;
 
 enum attend_kernel : uint32_t {
     attend_few,     // one block has the rows, its waves share out the keys
@@ -100,9 +101,36 @@ inline uint32_t attend_max_splits_of(const attend_plan& p, uint32_t n_kv, uint32
         {few, std::max(1u, tiles / attend_waves + (tiles % attend_waves != 0)), attend_max_splits}));
 }
 
+// The kernels for more than 16 rows of a KV head.
+inline void set_attend_kernel(attend_plan& p, attend_kernel kernel, uint64_t rows) {
+    p.kernel = kernel;
+    p.block_rows = kernel == attend_turns ? 256 : kernel == attend_many32 ? 128 : 64;
+    p.row_blocks = static_cast<uint32_t>((rows + p.block_rows - 1) / p.block_rows);
+}
+inline bool attend_takes(attend_kernel kernel, uint64_t rows, uint32_t hd, bool by_pairs) {
+    switch (kernel) {
+    case attend_turns:  // over 128 dims a wave's rows leave no second wave on a SIMD
+        return rows > 128 && hd <= 128 && !by_pairs;
+    case attend_many32:
+        return rows > 64 && !by_pairs;
+    default:
+        return true;
+    }
+}
+
 // n tokens of `group` query heads per KV head attend up to len keys. by_pairs:
 // a binary16 state whose K rows are off 16 bytes; its tiles go through
 // registers, which 32 rows a wave do not leave.
+//
+// The more rows a block has, the less of its tiles' cost each bears: 509
+// tokens of 4 heads behind 7683 (8 KV heads of 128) take the turns kernel 102
+// us and attend_many32 113. But where the blocks of all splits do not reach
+// the CUs' count, the time is one block's way through its few tiles, and
+// smaller blocks go it sooner: 29 tokens of 7 heads behind 171 took the turns
+// kernel 22.8 us and take attend_many16 11.2; 95 tokens of 4 heads behind 8,
+// 19.4 and 8.3. And where the last block's half would go without rows, which
+// leaves the turns kernel's other half no one to take turns with, the blocks
+// of attend_many32, at 1.1 times the time a row, can win.
 inline attend_plan plan_attend_rows(uint32_t n, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t len,
                                     bool by_pairs) {
     attend_plan p{};
@@ -110,17 +138,19 @@ inline attend_plan plan_attend_rows(uint32_t n, uint32_t group, uint32_t n_kv, u
     if (rows <= 16) {
         p.kernel = attend_few;
         p.block_rows = 16;
-    } else if (rows <= 64 || by_pairs) {
-        p.kernel = attend_many16;
-        p.block_rows = 64;
-    } else if (rows <= 128 || hd > 128) {  // over 128 dims a wave's rows leave no second wave on a SIMD
-        p.kernel = attend_many32;
-        p.block_rows = 128;
+        p.row_blocks = 1;
     } else {
-        p.kernel = attend_turns;
-        p.block_rows = 256;
+        for (const attend_kernel kernel : {attend_turns, attend_many32, attend_many16}) {
+            if (!attend_takes(kernel, rows, hd, by_pairs)) {
+                continue;
+            }
+            set_attend_kernel(p, kernel, rows);
+            const bool halved = kernel == attend_turns && (rows + 127) / 128 * 11 < uint64_t{p.row_blocks} * 2 * 10;
+            if (!halved && uint64_t{p.row_blocks} * n_kv * attend_max_splits_of(p, n_kv, len) >= attend_cus) {
+                break;
+            }
+        }
     }
-    p.row_blocks = static_cast<uint32_t>((rows + p.block_rows - 1) / p.block_rows);
     const uint32_t tiles = len / attend_tile + (len % attend_tile != 0);
     const uint32_t splits = attend_max_splits_of(p, n_kv, len);
     p.chunk = std::max(1u, (tiles + splits - 1) / splits);
@@ -134,18 +164,25 @@ inline uint64_t attend_scratch_floats(const attend_plan& p, uint32_t n_kv, uint6
     return p.splits > 1 ? uint64_t{p.splits} * n_kv * rows * (hd + 2) : 0;
 }
 
-// The most any call of up to max_n tokens on up to max_len keys needs: splits
-// only grow with the keys, and there are none from some count of rows on.
+// The most any call of up to max_n tokens on up to max_len keys needs: each
+// kernel's splits only grow with the keys, and there are none from some count
+// of rows on.
 inline uint64_t attend_scratch_bound(uint32_t max_n, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t max_len,
                                      bool by_pairs) {
     uint64_t most = 0;
     for (uint32_t n = 1; n <= max_n; ++n) {
-        const attend_plan p = plan_attend_rows(n, group, n_kv, hd, max_len, by_pairs);
         const uint64_t rows = uint64_t{n} * group;
         if (rows * n_kv > attend_split_waves * 64) {  // a wave's most rows: no splits from here on
             break;
         }
-        const uint32_t splits = attend_max_splits_of(p, n_kv, max_len);
+        attend_plan p{attend_few, 16, 1, 0, 0};
+        uint32_t splits = rows <= 16 ? attend_max_splits_of(p, n_kv, max_len) : 1;
+        for (const attend_kernel kernel : {attend_turns, attend_many32, attend_many16}) {
+            if (rows > 16 && attend_takes(kernel, rows, hd, by_pairs)) {
+                set_attend_kernel(p, kernel, rows);
+                splits = std::max(splits, attend_max_splits_of(p, n_kv, max_len));
+            }
+        }
         if (splits > 1) {
             most = std::max(most, splits * n_kv * rows * (hd + 2));
         }
