@@ -244,6 +244,50 @@ def test_larger_steps_of_unseen_keys(room, n_heads, n_kv, hd, n, pos, tree):
         assert_held(got[i:i + 1], want[i:i + 1], tol[i:i + 1], f"token {i}")
 
 
+# Calls whose blocks fill the CUs, so that rows go to the kernels of 32 rows a
+# wave: (query heads, KV heads, head size, tokens) behind some 800 keys.
+FULL = [(256, 64, 128, 33), (256, 64, 64, 50), (64, 64, 32, 200), (448, 64, 96, 37), (192, 64, 40, 61), (128, 64, 80, 100),
+        (128, 64, 128, 40), (128, 64, 160, 50), (128, 64, 256, 37), (64, 64, 224, 90)]
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,n", FULL)
+@pytest.mark.parametrize("kind", ["causal8", "tree8", "tree16"])
+def test_many_blocks(room, n_heads, n_kv, hd, n, kind):
+    """Growing V steps (8-bit), infinities and NaN among the drafted or later
+    rows, and NaN behind them; two of the KV heads checked."""
+    pos, group = 800 - n // 2, n_heads // n_kv
+    g = np.random.default_rng(hd + n)
+    eight = kind != "tree16"
+    x = g.standard_normal((2, pos + n, n_kv, hd)).astype(np.float32 if eight else np.float16)
+    if eight:
+        x[1, pos:] *= (2.0 ** np.linspace(-20, 20, n)).astype(np.float32)[:, None, None]
+        x[1, :pos] *= np.float32(2.0 ** -20)
+    for j, bad in ((n - 9, np.inf), (n - 7, -np.inf), (n - 5, np.nan)):
+        x[1, pos + j, n_kv - 1, j % hd] = bad
+    x[0, pos + n - 6, 0, 1] = np.nan
+    if eight:
+        cache = capi.kv8_state(room, pos + n + 70, n_kv, hd)
+        append8(room, cache, x[0], x[1], 0)
+    else:
+        cache = capi.kv_state(room, pos + n + 70, n_kv, hd)
+        vt = np.full((n_kv * hd, cache.ctx_stride), 0x7c00, np.uint16)
+        vt[:, :pos + n] = x[1].reshape(pos + n, -1).view(np.uint16).T
+        room.upload(cache.k_offset, np.ascontiguousarray(x[0]))
+        room.upload(cache.v_offset, vt)
+    q = g.standard_normal((n, n_heads * hd)).astype(np.float32)
+    mask = None if kind == "causal8" else capi.tree_mask([int(g.integers(max(-1, i - 4), i)) for i in range(n)])
+    sees = causal(n, pos) if mask is None else tree_sees(mask, n, pos)
+    got = attend_tree(room, cache, q, pos, n_heads, 0.125, mask) if not eight else \
+        attend8(room, cache, q, pos, n_heads, 0.125, mask=mask)
+    heads = [0, n_kv - 1]
+    some = [y.reshape(n, n_kv, group * hd)[:, heads].reshape(n, -1) for y in (q, got)]
+    k, v = ((values(y[:, heads]) if eight else y[:, heads].astype(np.float64)) for y in x)
+    want, tol = attend64(some[0], k, v, 2 * group, 0.125, sees)
+    assert np.isfinite(want).any() and not np.isfinite(want).all()
+    for i in range(n):
+        assert_held(some[1][i:i + 1], want[i:i + 1], tol[i:i + 1], f"token {i}")
+
+
 @pytest.mark.parametrize("n_heads,n_kv,hd,n", ROW_COUNTS)
 @pytest.mark.parametrize("eight", [False, True])
 def test_wild_rows_at_every_row_count(room, n_heads, n_kv, hd, n, eight):
