@@ -2,12 +2,15 @@
 // are outputs already divided by their sums, so the row is their mean,
 // weighted by sum * exp2(maximum - largest maximum).
 //
-// One wave per (KV head, query row) where there are many rows; where there
-// are few (a decode step), four, each a quarter of the head's dims. Every
+// One wave per (KV head, query row); where rows are few and one wave would
+// take its splits in several rounds of loads (a decode step), four, each a
+// quarter of the head's dims (32 rows of 17 splits 3.7 us, one wave 4.8; but 14
+// rows of 2 splits 3.8 and 3.1, and 3904 rows of 32 splits 8.4 and 7.4). Every
 // wave makes all the weights itself, four splits a lane, with no barrier; a
 // lane then sums every parts-th split of its quad of dims in order, and the
-// parts meet in a fixed tree. A few hundred KB to some MB from L2: bound by
-// the launch and two dependent trips.
+// parts meet in a fixed tree, so results do not depend on timing. A few
+// hundred KB to some MB from L2: bound by the launch and two dependent trips;
+// 16288 rows of 4 splits, 34 MB, take 10.9 us, 3.1 TB/s.
 
 #include "attend_rows.hpp"
 
@@ -95,12 +98,13 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(const attend_rows_arg
 
 hipError_t launch_attend_merge(const attend_rows_args& a, hipStream_t stream) {
     const uint64_t units = uint64_t{a.n} * a.group * a.n_kv;
-    const uint32_t wpr = units < 1024 && a.hd >= 16 ? 4 : 1;
-    const uint32_t all = (a.hd + 3) / 4;
     uint32_t quads = 1;
-    while (quads * wpr < all) {
+    while (quads * 4 < a.hd) {
         quads *= 2;
     }
+    const uint32_t round = 64 / quads * 4;  // splits that one wave loads at once
+    const uint32_t wpr = units < 1024 && a.splits > round && quads >= 4 ? 4 : 1;
+    quads /= wpr;
     const uint64_t blocks = (units * wpr + 3) / 4;
     if (blocks > 0x7fffffffu) {
         return hipErrorInvalidValue;

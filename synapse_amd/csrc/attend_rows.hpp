@@ -7,16 +7,22 @@
 // over the keys t that row r sees, in one pass with a running maximum m.
 //
 // Rows. The query rows of a KV head are (token, head) pairs, r = token *
-// group + head: a key or value byte serves all of them. Two kernels share the
-// arithmetic here:
-//  - up to 16 rows (a decode step): a wave takes all of them and every fourth
-//    tile of 64 keys of the block's split, straight from memory into operand
-//    registers, and the block's four waves meet in LDS at the end. Bound by
-//    HBM, so nothing is shared and no barrier is in the loop.
-//  - more rows: each of the four waves has 16 or 32 of its own, and the tiles
-//    of keys, which they all need, come through LDS as operands (two buffers,
-//    one barrier a tile). Bound by the matrix cores, the exponentials and
-//    LDS, which are about even at 32 rows a wave.
+// group + head: a key or value byte serves all of them. Three kernels share
+// the arithmetic here (plan_attend_rows chooses; 32 query heads on 8 KV heads
+// of 128 unless said otherwise):
+//  - up to 16 rows (a decode step), attend_few: a wave takes all of them and
+//    every fourth tile of 64 keys of the block's split, straight from memory
+//    into operand registers, and the block's four waves meet in LDS at the
+//    end. Bound by HBM, so nothing is shared and no barrier is in the loop:
+//    100001 keys in 39.7 us (5.3 TB/s); 4097 in 6.3, which is the launch and a
+//    chain of four trips to memory (q and tile, then three tiles).
+//  - more rows, attend_many: each of the four waves has 16 or 32 of its own,
+//    and the tiles of keys, which they all need, come through LDS as operands
+//    (two buffers, one barrier a tile). 26 tokens behind 4096: 15.3 us.
+//  - many rows, attend_turns: eight waves of 32, whose halves take turns at
+//    the matrix cores. 509 tokens behind 7683: 100.5 us (659 TFLOP/s counted,
+//    988 issued, as P V goes twice); 61 behind 20000: 42.2 us. The matrix
+//    units are 44 % busy and the vector units 48 %.
 // Splits of one row block meet in a second, small kernel (attend_merge.hip).
 //
 // Products. S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_16x16x32_f16: a
@@ -792,7 +798,7 @@ struct f16_source {
 
 // grid: KV heads x splits (one row block); block 256. Two waves per SIMD where
 // the registers allow it (8-bit heads of up to 128: 100001 keys of 8 x 128 in
-// 40.5 us, 5.2 TB/s; one wave 47.6).
+// 39.7 us; one wave 47.6).
 template <int DC, class SRC, bool TREE>
 __global__ __launch_bounds__(256, SRC::eight && DC <= 4 ? 2 : 1) void attend_few_kernel(const attend_rows_args a) {
     using namespace attend;
@@ -925,7 +931,7 @@ __global__ __launch_bounds__(256, SRC::eight && DC <= 4 ? 2 : 1) void attend_few
 }
 
 // ---- more rows: waves own rows, tiles come through LDS -------------------------
-// grid: splits x row blocks x KV heads; block 256. A buffer holds a tile as
+// grid: KV heads x splits x row blocks; block 256. A buffer holds a tile as
 // operands in lane order: K (st, dc), then V (dt, c), 1 KiB each, so every
 // LDS access is 64 neighbouring 16-byte units.
 template <int DC, int RT, bool EIGHT, bool WHOLE8, bool TREE>

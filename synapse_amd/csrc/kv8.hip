@@ -12,7 +12,9 @@
 // other) and are bound by HBM: a block takes one tile of 64 positions of one
 // KV head, a part-wave of hd / 4 lanes takes one row at a time, four values a
 // lane, and LDS turns rows into the tile's record and back, so that both
-// sides of the copy are whole lines.
+// sides of the copy are whole lines. 16384 rows of 8 x 128 f32: append 41.5 us
+// and read 34.1 us for 169 MB (4.1 and 5.0 TB/s); 100000 rows appended in 224 us
+// (4.6 TB/s); one row 3.7 and 2.8 us, the launch and a trip each way.
 
 #include "kernels.hpp"
 
@@ -350,7 +352,8 @@ struct read_rows {
 // first + i: every source is read before it is written over when a thread
 // owns its column (one word of K, one feature of V^T, one byte or step) and
 // goes through the rows in order, `batch` loads ahead of their stores. A
-// handful of rows of a few KB: bound by two dependent trips to memory.
+// handful of rows of a few KB: bound by the launch and two dependent trips to
+// memory (6 rows: 3.3 us, of an 8-bit state 4.3).
 constexpr uint32_t batch = 8;
 
 // A launch of up to `batch` rows (an accepted path) carries them in an argument
