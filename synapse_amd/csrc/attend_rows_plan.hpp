@@ -101,7 +101,14 @@ inline uint32_t attend_max_splits_of(const attend_plan& p, uint32_t n_kv, uint32
         {few, std::max(1u, tiles / attend_waves + (tiles % attend_waves != 0)), attend_max_splits}));
 }
 
-// The kernels for more than 16 rows of a KV head.
+// Up to 16 rows of a KV head go to attend_few, but over a binary16 state of
+// more than 192 dims, whose tile spills its registers: 16 rows of 4 heads of
+// 256 behind 12000 keys 26.0 us, by attend_many16 22.0 (of 192 18.1 and 18.8; over
+// an 8-bit state of 256 18.9 and 20.5).
+inline bool attend_takes_few(uint64_t rows, uint32_t hd, bool halves) {
+    return rows <= 16 && !(halves && hd > 192);
+}
+// The kernels for other rows.
 inline void set_attend_kernel(attend_plan& p, attend_kernel kernel, uint64_t rows) {
     p.kernel = kernel;
     p.block_rows = kernel == attend_turns ? 256 : kernel == attend_many32 ? 128 : 64;
@@ -118,9 +125,9 @@ inline bool attend_takes(attend_kernel kernel, uint64_t rows, uint32_t hd, bool 
     }
 }
 
-// n tokens of `group` query heads per KV head attend up to len keys. by_pairs:
-// a binary16 state whose K rows are off 16 bytes; its tiles go through
-// registers, which 32 rows a wave do not leave.
+// n tokens of `group` query heads per KV head attend up to len keys. halves: a
+// binary16 state; by_pairs: one whose K rows are off 16 bytes; its tiles go
+// through registers, which 32 rows a wave do not leave.
 //
 // The more rows a block has, the less of its tiles' cost each bears: 509
 // tokens of 4 heads behind 7683 (8 KV heads of 128) take the turns kernel 102
@@ -132,10 +139,10 @@ inline bool attend_takes(attend_kernel kernel, uint64_t rows, uint32_t hd, bool 
 // leaves the turns kernel's other half no one to take turns with, the blocks
 // of attend_many32, at 1.1 times the time a row, can win.
 inline attend_plan plan_attend_rows(uint32_t n, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t len,
-                                    bool by_pairs) {
+                                    bool halves, bool by_pairs) {
     attend_plan p{};
     const uint64_t rows = uint64_t{n} * group;
-    if (rows <= 16) {
+    if (attend_takes_few(rows, hd, halves)) {
         p.kernel = attend_few;
         p.block_rows = 16;
         p.row_blocks = 1;
@@ -168,7 +175,7 @@ inline uint64_t attend_scratch_floats(const attend_plan& p, uint32_t n_kv, uint6
 // kernel's splits only grow with the keys, and there are none from some count
 // of rows on.
 inline uint64_t attend_scratch_bound(uint32_t max_n, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t max_len,
-                                     bool by_pairs) {
+                                     bool halves, bool by_pairs) {
     uint64_t most = 0;
     for (uint32_t n = 1; n <= max_n; ++n) {
         const uint64_t rows = uint64_t{n} * group;
@@ -176,9 +183,10 @@ inline uint64_t attend_scratch_bound(uint32_t max_n, uint32_t group, uint32_t n_
             break;
         }
         attend_plan p{attend_few, 16, 1, 0, 0};
-        uint32_t splits = rows <= 16 ? attend_max_splits_of(p, n_kv, max_len) : 1;
+        const bool few = attend_takes_few(rows, hd, halves);
+        uint32_t splits = few ? attend_max_splits_of(p, n_kv, max_len) : 1;
         for (const attend_kernel kernel : {attend_turns, attend_many32, attend_many16}) {
-            if (rows > 16 && attend_takes(kernel, rows, hd, by_pairs)) {
+            if (!few && attend_takes(kernel, rows, hd, by_pairs)) {
                 set_attend_kernel(p, kernel, rows);
                 splits = std::max(splits, attend_max_splits_of(p, n_kv, max_len));
             }

@@ -11,7 +11,10 @@ template <int DC, bool WHOLE8>
 hipError_t by_rows(const attend_rows_args& a, hipStream_t stream) {
     switch (a.kernel) {
     case attend_few:
-        return launch_attend_blocks(attend_few_kernel<DC, attend::f16_source<DC, WHOLE8>, true>, 256, a, stream);
+        if constexpr (DC <= 6) {
+            return launch_attend_blocks(attend_few_kernel<DC, attend::f16_source<DC, WHOLE8>, true>, 256, a, stream);
+        }
+        return hipErrorInvalidValue;
     case attend_many16:
         return launch_attend_blocks(attend_many_kernel<DC, 1, false, WHOLE8, true>, 256, a, stream);
     case attend_many32:

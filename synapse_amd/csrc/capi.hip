@@ -470,14 +470,14 @@ int check_mask(const syn_arena* a, uint64_t offset, uint32_t n, span& at) {
 // the scratch, and the operands' places.
 int fill_attend_rows(syn_arena* a, syn::attend_rows_args& r, uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t n,
                      uint32_t pos, float scale, uint32_t q_dtype, uint64_t q_offset, uint64_t out_offset,
-                     uint64_t scratch_offset, uint64_t scratch_bytes, uint64_t mask_offset, bool by_pairs,
+                     uint64_t scratch_offset, uint64_t scratch_bytes, uint64_t mask_offset, bool halves, bool by_pairs,
                      std::initializer_list<span> state, const char* call) {
     const uint32_t group = n_heads / n_kv;
     const uint64_t rows = uint64_t{n} * group;
     if (rows > 0x7fffffffu) {
         return fail(SYN_HIP_EUNSUPPORTED, "%s: %u tokens of %u heads per KV head", call, n, group);
     }
-    const syn::attend_plan p = syn::plan_attend_rows(n, group, n_kv, hd, pos + n, by_pairs);
+    const syn::attend_plan p = syn::plan_attend_rows(n, group, n_kv, hd, pos + n, halves, by_pairs);
     if (p.row_blocks > syn::attend_max_row_blocks || group > syn::attend_max_group) {
         return fail(SYN_HIP_EUNSUPPORTED, "%s: %u tokens of %u heads per KV head", call, n, group);
     }
@@ -531,11 +531,12 @@ int fill_attend_rows(syn_arena* a, syn::attend_rows_args& r, uint32_t n_heads, u
 }
 
 uint64_t attend_rows_scratch(uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t max_ctx, uint32_t max_batch,
-                             bool by_pairs) {
+                             bool halves, bool by_pairs) {
     if (n_heads == 0 || !kv8_shape_ok(max_ctx, n_kv, hd) || n_heads % n_kv != 0) {
         return 0;
     }
-    return align256(syn::attend_scratch_bound(std::min(max_batch, max_ctx), n_heads / n_kv, n_kv, hd, max_ctx, by_pairs) *
+    return align256(syn::attend_scratch_bound(std::min(max_batch, max_ctx), n_heads / n_kv, n_kv, hd, max_ctx, halves,
+                                              by_pairs) *
                     4);
 }
 
@@ -581,7 +582,7 @@ int fill_kv8_attend(syn_arena* a, const syn_kv8_attn_desc* d, syn::attend_rows_a
     const syn_kv8_desc& c = d->cache;
     if (int e = fill_attend_rows(a, r, d->n_heads, c.n_kv_heads, c.head_dim, d->n, d->pos, d->scale, d->q_dtype,
                                  d->q_offset, d->out_offset, d->scratch_offset, d->scratch_bytes, d->mask_offset,
-                                 false, {kv8_span(c)}, "kv8 attention")) {
+                                 false, false, {kv8_span(c)}, "kv8 attention")) {
         return e;
     }
     const syn::kv8_shape s = syn::kv8_shape_of(c.max_ctx, c.n_kv_heads, c.head_dim);
@@ -1597,12 +1598,12 @@ int syn_hip_kv8_read(syn_arena* a, const syn_kv8_desc* cache, uint64_t k_out, ui
 
 uint64_t syn_hip_kv8_attention_scratch_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
                                              uint32_t max_ctx, uint32_t max_batch) {
-    return attend_rows_scratch(n_heads, n_kv_heads, head_dim, max_ctx, max_batch, false);
+    return attend_rows_scratch(n_heads, n_kv_heads, head_dim, max_ctx, max_batch, false, false);
 }
 
 uint64_t syn_hip_attend_tree_scratch_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
                                            uint32_t max_ctx, uint32_t max_batch) {
-    return attend_rows_scratch(n_heads, n_kv_heads, head_dim, max_ctx, max_batch, head_dim % 8 != 0);
+    return attend_rows_scratch(n_heads, n_kv_heads, head_dim, max_ctx, max_batch, true, head_dim % 8 != 0);
 }
 
 int syn_hip_kv8_attend(syn_arena* a, const syn_kv8_attn_desc* d) {
@@ -1647,7 +1648,7 @@ int syn_hip_attend_tree(syn_arena* a, const syn_attn_desc* d, uint64_t mask_offs
     syn::attend_rows_args r{};
     if (int e = fill_attend_rows(a, r, d->n_heads, c.n_kv_heads, c.head_dim, d->n, d->pos, d->scale, d->q_dtype,
                                  d->q_offset, d->out_offset, d->scratch_offset, d->scratch_bytes, mask_offset,
-                                 c.head_dim % 8 != 0,
+                                 true, c.head_dim % 8 != 0,
                                  {{c.k_offset, uint64_t{c.max_ctx} * row * 2, "the state's K"},
                                   {c.v_offset, row * c.ctx_stride * 2, "the state's V^T"}},
                                  "attend_tree")) {

@@ -41,18 +41,19 @@ int main() {
         const uint32_t group = upto(40), n_kv = upto(64), hd = 2 * upto(128), max_ctx = upto(300000);
         const uint32_t n = upto(max_ctx), max_n = n + upto(100) - 1;
         const uint32_t len = n + (max_ctx > n ? static_cast<uint32_t>(r()) % (max_ctx - n + 1) : 0);
-        const bool by_pairs = i % 3 == 0;
-        const syn::attend_plan p = syn::plan_attend_rows(n, group, n_kv, hd, len, by_pairs);
+        const bool by_pairs = i % 3 == 0, halves = by_pairs || i % 3 == 1;
+        const syn::attend_plan p = syn::plan_attend_rows(n, group, n_kv, hd, len, halves, by_pairs);
         CHECK(!by_pairs || p.kernel <= syn::attend_many16);
         CHECK(p.kernel != syn::attend_turns || hd <= 128);
         CHECK(p.kernel != syn::attend_few || p.row_blocks == 1);
+        CHECK(p.kernel != syn::attend_few || !halves || hd <= 192);
         CHECK(uint64_t{p.row_blocks} * p.block_rows >= uint64_t{n} * group);
         CHECK(uint64_t{p.row_blocks - 1} * p.block_rows < uint64_t{n} * group);
         const uint32_t tiles = (len + 63) / 64;
         CHECK(uint64_t{p.chunk} * p.splits >= tiles && uint64_t{p.chunk} * (p.splits - 1) < tiles);
         CHECK(p.splits >= 1 && p.splits <= syn::attend_max_splits);
         CHECK(syn::attend_scratch_floats(p, n_kv, uint64_t{n} * group, hd) <=
-              syn::attend_scratch_bound(std::min(max_n, max_ctx), group, n_kv, hd, max_ctx, by_pairs));
+              syn::attend_scratch_bound(std::min(max_n, max_ctx), group, n_kv, hd, max_ctx, halves, by_pairs));
     }
     CHECK_DONE();
 }
